@@ -653,6 +653,92 @@ int pxg_h5_basecall_many(int64_t n, const pxg_h5* const* files, const int64_t* i
                          uint8_t* qual_arena, const int64_t* move_start, const int64_t* n_moves,
                          uint8_t* move_arena, int32_t threads, int32_t* status);
 
+/* ---- operators on the caller's device memory (sequence layers and their training) --------------------------------
+ * Every pointer below is device memory of the CURRENT HIP device; `stream` is a hipStream_t of that device (NULL: its
+ * default stream).  The calls only launch kernels: no allocation, no synchronisation, no memset, so they may be captured
+ * into a graph.  Work that needs scratch memory takes it from the caller (`workspace`, at least as many bytes as the
+ * *_workspace_bytes function says, not shared by calls that may run at once); its contents before and after mean nothing.
+ * Values are checked where the host can see them (shapes, types, pointers): PXG_E_INVALID; what lies in device memory
+ * (lengths, class indices) is bounded by the kernels themselves.  No context is needed; calls from several threads are
+ * independent of each other. */
+enum pxg_dtype { PXG_DT_F32 = 0, PXG_DT_BF16 = 1, PXG_DT_F16 = 2 };
+
+#define PXG_DECAY_MAX_WIDTH 128    /* largest dk and dv */
+#define PXG_TOP_MAX_K       128    /* largest k of the top logits */
+
+/* A [batch][step][head][width] tensor: width is contiguous, the other strides are free (in elements, 0 for a broadcast). */
+typedef struct {
+    const void* data;
+    int64_t batch_stride, step_stride, head_stride;
+} pxg_sequence;
+
+/* Linear attention with one decay a_h = exp(log_decay[h]) per head, a recurrence over the steps of each sequence:
+ *     S_t = a_h S_(t-1) + k_t v_t^T        o_t = q_t S_t        S_(-1) = initial_state (0 where NULL)
+ * Steps at or behind lengths[b] are neither read nor part of the state; their rows of `out` and of the gradients are 0.
+ * A length below 0 counts as 0, one above `steps` as `steps`. */
+typedef struct {
+    uint32_t struct_bytes;            /* sizeof(pxg_decay) */
+    int32_t dtype;                    /* pxg_dtype of q, k, v, out, grad_out and the gradients of q, k, v */
+    int64_t batch, steps;
+    int32_t heads, dk, dv;
+    int32_t lengths_are_64;           /* lengths: int64_t instead of int32_t */
+    pxg_sequence q, k, v;
+    const float* log_decay;           /* [heads] */
+    const void* lengths;              /* [batch] or NULL: every sequence has `steps` steps */
+    const float* initial_state;       /* [batch][heads][dk][dv] or NULL */
+    void* out;                        /* [batch][steps][heads][dv] */
+    float* final_state;               /* [batch][heads][dk][dv] or NULL */
+    /* pxg_decay_backward only */
+    pxg_sequence grad_out;            /* data may be NULL: all zero */
+    const float* grad_final_state;    /* or NULL */
+    void *grad_q, *grad_k, *grad_v;   /* contiguous like q, k, v */
+    float* grad_log_decay;            /* [heads] or NULL: not wanted */
+    float* grad_initial_state;        /* or NULL: not wanted */
+    void* workspace;
+    int64_t workspace_bytes;
+} pxg_decay;
+
+int64_t pxg_decay_workspace_bytes(const pxg_decay* call, int32_t backward);
+int pxg_decay_forward(const pxg_decay* call, void* stream);
+int pxg_decay_backward(const pxg_decay* call, void* stream);
+/* One step of the recurrence for every sequence: `final_state` is read and updated in place, q / k / v and `out` hold one
+ * step (steps = 1).  `lengths`, if given, is uint8_t[batch]: a sequence whose byte is 0 keeps its state, its row of `out` is 0. */
+int pxg_decay_step(const pxg_decay* call, void* stream);
+
+/* The k largest of each row's `classes` logits in descending order (ties: lowest class first; NaN counts as the largest),
+ * their classes, and rest[row] = log sum over the OTHER classes of exp(logit / temperature) (-inf where there is none). */
+int pxg_top_logits(int32_t dtype, int64_t rows, int64_t classes, const void* logits, int64_t row_stride, int32_t k,
+                   float temperature, void* values, int32_t* indices, float* rest, void* stream);
+
+/* Distillation from such a teacher: p = softmax over [values / temperature, rest] (the unlisted classes are one class more;
+ * rest NULL: the listed ones are all there is), q = the student's softmax(logits / temperature) over the same k + 1 classes;
+ *     row_loss[n] = weight[n] temperature^2 sum p (log p - log q),       loss = sum of row_loss / (mean ? rows : 1)
+ * An index of -1 is an empty place; a class listed more than once gets the sum of its shares; an index outside the classes
+ * makes its row's loss and gradient NaN.  Rows of weight 0 and rows with nothing listed and no rest give 0 whatever they hold. */
+typedef struct {
+    uint32_t struct_bytes;            /* sizeof(pxg_distill) */
+    int32_t dtype;                    /* pxg_dtype of logits and grad_logits */
+    int64_t rows, classes, row_stride;
+    const void* logits;
+    int32_t k, value_dtype;           /* pxg_dtype of values */
+    const void* values;               /* [rows][k] */
+    const void* indices;              /* [rows][k] */
+    const float* rest;                /* [rows] or NULL */
+    const float* weight;              /* [rows] or NULL: 1 */
+    float temperature;
+    int32_t indices_are_64;
+    int32_t mean;
+    int32_t grad_per_row;             /* backward: grad_loss is [rows] (of row_loss) instead of one value (of loss) */
+    float* row_loss;                  /* [rows] */
+    float* loss;                      /* one value, or NULL: not wanted */
+    float* stats;                     /* [rows][4]: what the backward pass needs of the forward pass */
+    const float* grad_loss;
+    void* grad_logits;                /* [rows][classes] contiguous */
+} pxg_distill;
+
+int pxg_distill_forward(const pxg_distill* call, void* stream);
+int pxg_distill_backward(const pxg_distill* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

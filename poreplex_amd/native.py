@@ -25,6 +25,8 @@ PXG_MAX_CLASSES = 8
 PXG_MAX_CALIBRATION = 64
 UNSPLIT_E_GEOMETRY = -3
 UNSPLIT_E_WINDOW = -4
+PXG_DECAY_MAX_WIDTH = 128
+PXG_TOP_MAX_K = 128
 
 STATUS_NAMES = (
     'okay', 'disappeared', 'irregular_fast5', 'scaler_signal_too_short',
@@ -175,6 +177,31 @@ class PxgDeviceInfo(C.Structure):
                 ('compute_units', C.c_int32), ('wavefront_size', C.c_int32),
                 ('total_mem', C.c_int64), ('lds_per_cu', C.c_int32),
                 ('clock_khz', C.c_int32)]
+
+
+class PxgSequence(C.Structure):            # pxg_sequence
+    _fields_ = [('data', C.c_void_p), ('batch_stride', C.c_int64), ('step_stride', C.c_int64), ('head_stride', C.c_int64)]
+
+
+class PxgDecay(C.Structure):               # pxg_decay
+    _fields_ = [('struct_bytes', C.c_uint32), ('dtype', C.c_int32), ('batch', C.c_int64), ('steps', C.c_int64),
+                ('heads', C.c_int32), ('dk', C.c_int32), ('dv', C.c_int32), ('lengths_are_64', C.c_int32),
+                ('q', PxgSequence), ('k', PxgSequence), ('v', PxgSequence),
+                ('log_decay', C.c_void_p), ('lengths', C.c_void_p), ('initial_state', C.c_void_p),
+                ('out', C.c_void_p), ('final_state', C.c_void_p),
+                ('grad_out', PxgSequence), ('grad_final_state', C.c_void_p),
+                ('grad_q', C.c_void_p), ('grad_k', C.c_void_p), ('grad_v', C.c_void_p),
+                ('grad_log_decay', C.c_void_p), ('grad_initial_state', C.c_void_p),
+                ('workspace', C.c_void_p), ('workspace_bytes', C.c_int64)]
+
+
+class PxgDistill(C.Structure):             # pxg_distill
+    _fields_ = [('struct_bytes', C.c_uint32), ('dtype', C.c_int32), ('rows', C.c_int64), ('classes', C.c_int64),
+                ('row_stride', C.c_int64), ('logits', C.c_void_p), ('k', C.c_int32), ('value_dtype', C.c_int32),
+                ('values', C.c_void_p), ('indices', C.c_void_p), ('rest', C.c_void_p), ('weight', C.c_void_p),
+                ('temperature', C.c_float), ('indices_are_64', C.c_int32), ('mean', C.c_int32), ('grad_per_row', C.c_int32),
+                ('row_loss', C.c_void_p), ('loss', C.c_void_p), ('stats', C.c_void_p), ('grad_loss', C.c_void_p),
+                ('grad_logits', C.c_void_p)]
 
 
 # numpy views of the POD records (same layout, checked against ctypes sizes)
@@ -471,6 +498,15 @@ _SIGNATURES = {
                             C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p]),
     'pxg_detect_events': (C.c_int, [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p,
                                     C.c_int64, C.c_void_p, C.c_void_p]),
+    # operators on the caller's device memory (torch_ops.py)
+    'pxg_decay_workspace_bytes': (C.c_int64, [C.POINTER(PxgDecay), C.c_int32]),
+    'pxg_decay_forward': (C.c_int, [C.POINTER(PxgDecay), C.c_void_p]),
+    'pxg_decay_backward': (C.c_int, [C.POINTER(PxgDecay), C.c_void_p]),
+    'pxg_decay_step': (C.c_int, [C.POINTER(PxgDecay), C.c_void_p]),
+    'pxg_top_logits': (C.c_int, [C.c_int32, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int32, C.c_float, C.c_void_p,
+                                 C.c_void_p, C.c_void_p, C.c_void_p]),
+    'pxg_distill_forward': (C.c_int, [C.POINTER(PxgDistill), C.c_void_p]),
+    'pxg_distill_backward': (C.c_int, [C.POINTER(PxgDistill), C.c_void_p]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 TEXT_SYMBOLS = tuple(_TEXT_SIGNATURES)

@@ -1,0 +1,785 @@
+"""poreplex_amd/torch_ops.py against plain 64-bit statements of the same formulas.
+
+Tolerances.  A result of type t is rounded once: eps(t) / 2 of its value.  What is summed in float32 errs by at most
+(number of roundings on the way) * 2^-24 of the sum of the ABSOLUTE terms, which the statements below compute beside the value
+(`size`).  Half-precision results may also take products of operands that were split into two bfloat16 numbers: what is left over
+is at most 2^-18 of each term, for the weights inside a chunk and for the state (together 2^-17)."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip('torch')
+
+from poreplex_amd import native as N  # noqa: E402
+from poreplex_amd import torch_ops as ops  # noqa: E402
+
+F64 = torch.float64
+TYPES = {'f32': torch.float32, 'bf16': torch.bfloat16, 'f16': torch.float16}
+gpu = pytest.mark.gpu
+
+
+# ---- plain statements, 64 bits, on the CPU --------------------------------------------------------------------------
+def recurrence(q, k, v, log_decay, lengths=None, initial_state=None):
+    """(o, state), step after step."""
+    b, t, h, dk = q.shape
+    a = torch.exp(log_decay)[:, None, None]
+    state = torch.zeros(b, h, dk, v.shape[-1], dtype=F64) if initial_state is None else initial_state
+    rows = []
+    for i in range(t):
+        live = torch.ones(b, dtype=torch.bool) if lengths is None else i < lengths
+        live = live[:, None, None, None]
+        state = torch.where(live, a * state + k[:, i, :, :, None] * v[:, i, :, None, :], state)
+        rows.append(torch.where(live, q[:, i, :, :, None] * state, torch.zeros((), dtype=F64)).sum(-2))
+    out = torch.stack(rows, 1) if rows else torch.zeros(v.shape, dtype=F64)
+    return out, state
+
+
+def roundings(steps):
+    """on the way of one value: the terms inside a chunk of 64 steps, the width of the states, three for each chunk passed, the
+    decay factors"""
+    return 64 + 128 + 3 * (steps // 64 + 1) + 64
+
+
+def assert_near(got, want, size, steps, split=True, more=0.0):
+    dtype = got.dtype
+    tol = torch.finfo(dtype).eps / 2 * want.abs() + roundings(steps) * 2.0 ** -24 * size
+    if dtype != torch.float32 and split:
+        tol = tol + 2.0 ** -17 * size
+    if dtype == torch.float16:
+        tol = tol + 2.0 ** -25                      # half the least step of float16
+    tol = tol * (1 + 2.0 ** -7) + more + 1e-37
+    off = (got.double().cpu() - want).abs()
+    worst = (off - tol).max() if off.numel() else torch.tensor(-1.0)
+    assert torch.isfinite(got).all() and worst <= 0, 'off by up to {:.3g}, {:.3g} over'.format(float(off.max()), float(worst))
+
+
+def problem(b, t, h, dk, dv, dtype, ragged=False, state=False, seed=0, spans=(1.0, 8.0)):
+    g = torch.Generator().manual_seed(seed + 7 * t + dk)
+    n = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    dt = TYPES[dtype]
+    p = {'q': (n(b, t, h, dk) * dk ** -0.5).to(dt), 'k': n(b, t, h, dk).to(dt), 'v': n(b, t, h, dv).to(dt)}
+    p['log_decay'] = torch.log1p(-torch.exp2(-torch.linspace(*spans, h)))
+    p['lengths'] = None
+    if ragged:
+        p['lengths'] = torch.randint(0, t + 1, (b,), generator=g)
+        p['lengths'][0] = t
+        if b > 1:
+            p['lengths'][1] = 0
+        if b > 2:
+            p['lengths'][2] = min(1, t)
+    p['initial_state'] = n(b, h, dk, dv) if state else None
+    p['grad_out'], p['grad_state'] = n(b, t, h, dv).to(dt), n(b, h, dk, dv) if state else None
+    return p
+
+
+def to_f64(p):
+    return {x: (y.double() if y is not None and y.is_floating_point() else y) for x, y in p.items()}
+
+
+def to_gpu(p):
+    return {x: (None if y is None else y.cuda()) for x, y in p.items()}
+
+
+ARGS = ('q', 'k', 'v', 'log_decay', 'lengths', 'initial_state')
+LEAVES = ('q', 'k', 'v', 'log_decay', 'initial_state')
+
+
+def gradients(p):
+    """of sum(o * grad_out) + sum(state * grad_state), through the recurrence, for every leaf."""
+    p = to_f64(p)
+    leaves = [p[x].clone().requires_grad_() for x in LEAVES if p[x] is not None]
+    named = dict(zip([x for x in LEAVES if p[x] is not None], leaves))
+    out, state = recurrence(*[named.get(x, p[x]) for x in ARGS])
+    loss = (out * p['grad_out']).sum()
+    if p['grad_state'] is not None:
+        loss = loss + (state * p['grad_state']).sum()
+    return dict(zip(named, torch.autograd.grad(loss, leaves)))
+
+
+def absolute(p):
+    """the same problem with every operand's absolute value: its results are the sums of the absolute terms"""
+    return {x: (y.abs() if y is not None and y.is_floating_point() and x != 'log_decay' else y) for x, y in p.items()}
+
+
+# (batch, steps, heads, dk, dv): one step to several chunks, chunk borders, widths that are no multiple of anything
+SHAPES = [(1, 1, 1, 16, 16), (2, 5, 3, 8, 24), (3, 63, 2, 16, 16), (2, 64, 2, 32, 32), (2, 65, 1, 64, 64), (1, 130, 2, 48, 80),
+          (2, 200, 1, 128, 128), (3, 100, 2, 7, 13), (2, 129, 2, 1, 1), (1, 70, 1, 33, 128), (1, 300, 4, 16, 16), (2, 67, 1, 100, 20)]
+
+
+def test_plain_statement_against_differences():
+    """the 64-bit gradients against central differences, along one direction for each leaf"""
+    p = to_f64(problem(3, 12, 2, 4, 5, 'f32', ragged=True, state=True))
+    grads = gradients(p)
+
+    def value(q):
+        out, state = recurrence(*[q[x] for x in ARGS])
+        return float((out * q['grad_out']).sum() + (state * q['grad_state']).sum())
+    g = torch.Generator().manual_seed(3)
+    for x in LEAVES:
+        d = torch.randn(p[x].shape, generator=g, dtype=F64)
+        e = 1e-5
+        up, down = dict(p), dict(p)
+        up[x], down[x] = p[x] + e * d, p[x] - e * d
+        want = float((grads[x] * d).sum())
+        # third derivatives are of the size of the values, times e^2; rounding 1e-16 / e
+        assert abs((value(up) - value(down)) / (2 * e) - want) < 1e-6 * (1 + abs(want)), x
+
+
+@gpu
+@pytest.mark.parametrize('dtype', sorted(TYPES))
+@pytest.mark.parametrize('ragged,state', [(False, False), (True, True)])
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+def test_decay_attention(shape, ragged, state, dtype):
+    p = problem(*shape, dtype, ragged, state)
+    out, final = ops.decay_attention(**{x: y for x, y in to_gpu(p).items() if x in ARGS}, return_state=True)
+    assert out.dtype == p['v'].dtype and final.dtype == torch.float32
+    want, want_state = recurrence(*[to_f64(p)[x] for x in ARGS])
+    size, size_state = recurrence(*[to_f64(absolute(p))[x] for x in ARGS])
+    assert_near(out, want, size, shape[1])
+    assert_near(final, want_state, size_state, shape[1])
+    if ragged:
+        for i, n in enumerate(p['lengths'].tolist()):
+            assert (out[i, n:] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize('dtype', sorted(TYPES))
+@pytest.mark.parametrize('ragged,state', [(False, False), (True, True)])
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+def test_decay_attention_gradients(shape, ragged, state, dtype):
+    p = problem(*shape, dtype, ragged, state, seed=1)
+    d = to_gpu(p)
+    leaves = [d[x].requires_grad_() for x in LEAVES if d[x] is not None]
+    out, final = ops.decay_attention(**{x: d[x] for x in ARGS}, return_state=True)
+    outs, grads = ([out, final], [d['grad_out'], d['grad_state']]) if state else ([out], [d['grad_out']])
+    got = dict(zip([x for x in LEAVES if d[x] is not None], torch.autograd.grad(outs, leaves, grads)))
+    check_gradients(got, p, shape)
+    again = ops.decay_attention_backward(d['grad_out'], *[d[x] for x in ARGS], grad_state=d['grad_state'])
+    for x, y in zip(LEAVES, again):
+        assert (y is None) == (x not in got) and (y is None or torch.equal(y, got[x])), x
+
+
+def check_gradients(got, p, shape):
+    want, size = gradients(p), gradients(absolute(p))
+    assert set(got) == set(want)
+    for x in got:
+        # what reaches log_decay is summed over the batch and over the steps, each weighted by its distance
+        n = shape[1] + (4 * shape[0] * shape[1] if x == 'log_decay' else 0)
+        assert got[x].dtype == p[x].dtype and got[x].shape == p[x].shape
+        assert_near(got[x], want[x], size[x].abs(), n)
+
+
+@gpu
+def test_decay_attention_gradients_against_differences():
+    """Directional central differences of the operator's own float32 result.  With a step of e the difference errs by the result's
+    rounding over 2 e and by e^2 / 6 of the third derivative along the direction, both of the size of the absolute terms."""
+    p = problem(2, 150, 2, 16, 24, 'f32', ragged=True, state=True, seed=2)
+    d, grads = to_gpu(p), {}
+    value = lambda q: float((torch.cat([(o.double() * g.double()).flatten() for o, g in zip(  # noqa: E731
+        ops.decay_attention(**{x: q[x] for x in ARGS}, return_state=True), (q['grad_out'], q['grad_state']))])).sum())
+    grads = dict(zip(LEAVES, ops.decay_attention_backward(d['grad_out'], *[d[x] for x in ARGS], grad_state=d['grad_state'])))
+    size = sum(float((o * g).sum()) for o, g in zip(recurrence(*[to_f64(absolute(p))[x] for x in ARGS]),
+                                                    (to_f64(absolute(p))['grad_out'], to_f64(absolute(p))['grad_state'])))
+    e = 2.0 ** -7
+    for x in LEAVES:
+        g = torch.Generator().manual_seed(5)
+        direction = torch.randn(p[x].shape, generator=g).cuda()
+        if x == 'log_decay':
+            direction = direction.abs() * p[x].abs().cuda()               # keeps the decay below 1
+        up, down = dict(d), dict(d)
+        up[x], down[x] = d[x] + e * direction, d[x] - e * direction
+        got, want = (value(up) - value(down)) / (2 * e), float((grads[x].double() * direction.double()).sum())
+        # linear in every leaf but log_decay, where the third derivative is bounded by 27 windows' worth of the terms
+        assert abs(got - want) <= roundings(150) * 2.0 ** -24 * size / e * 2 + (27 * e * e * size if x == 'log_decay' else 0), x
+
+
+@gpu
+@pytest.mark.parametrize('dtype', sorted(TYPES))
+def test_decay_attention_layouts(dtype):
+    """strides of every kind give what contiguous copies give, bit for bit: heads before steps, slices of a packed tensor (an odd
+    offset: no alignment), heads that share k and v, a batch that shares q"""
+    b, t, h, dk, dv = 2, 140, 3, 16, 32
+    p = to_gpu(problem(b, t, h, dk, dv, dtype, True, True, seed=3))
+    packed = torch.randn(b, t, h, 2 * dk + dv + 3, device='cuda').to(TYPES[dtype])
+    one_k, one_v = p['k'][:, :, :1].expand(b, t, h, dk), p['v'][:, :, :1].expand(b, t, h, dv)
+    variants = [
+        (p['q'].transpose(1, 2).contiguous().transpose(1, 2), p['k'].permute(2, 1, 0, 3).contiguous().permute(2, 1, 0, 3), p['v']),
+        (packed[..., 1:1 + dk], packed[..., 1 + dk:1 + 2 * dk], packed[..., 1 + 2 * dk:1 + 2 * dk + dv]),
+        (p['q'][:1].expand(b, t, h, dk), one_k, one_v),
+        (p['q'].transpose(2, 3).contiguous().transpose(2, 3), p['k'], p['v']),
+    ]
+    go = p['grad_out'].transpose(1, 2).contiguous().transpose(1, 2)
+    rest = [p['log_decay'], p['lengths'].int(), p['initial_state']]
+    for q, k, v in variants:
+        flat = [x.contiguous() for x in (q, k, v)]
+        for x, y in zip(ops.decay_attention(q, k, v, *rest, return_state=True), ops.decay_attention(*flat, *rest, return_state=True)):
+            assert torch.equal(x, y)
+        for x, y in zip(ops.decay_attention_backward(go, q, k, v, *rest, grad_state=p['grad_state']),
+                        ops.decay_attention_backward(p['grad_out'], *flat, *rest, grad_state=p['grad_state'])):
+            assert torch.equal(x, y)
+    # gradients of what the heads share are summed over them
+    k1 = p['k'][:, :, :1].clone().requires_grad_()
+    out = ops.decay_attention(p['q'], k1.expand(b, t, h, dk), one_v, *rest)
+    shared = torch.autograd.grad(out, k1, p['grad_out'])[0]
+    each = ops.decay_attention_backward(p['grad_out'], p['q'], one_k, one_v, *rest)[1]
+    assert torch.allclose(shared.float(), each.sum(2, keepdim=True).float(), rtol=2 * torch.finfo(TYPES[dtype]).eps, atol=1e-6)
+
+
+@gpu
+@pytest.mark.parametrize('dtype', sorted(TYPES))
+def test_decay_attention_padding_is_not_read(dtype):
+    """NaN and inf behind the lengths change nothing, in the results or in the gradients; lengths out of range are clamped"""
+    p = to_gpu(problem(4, 150, 2, 32, 16, dtype, state=True, seed=4))
+    p['lengths'] = torch.tensor([150, 0, 65, 130], device='cuda')
+    args = [p[x] for x in ARGS]
+    want = ops.decay_attention(*args, return_state=True) + ops.decay_attention_backward(p['grad_out'], *args, grad_state=p['grad_state'])
+    dirty = {x: p[x].clone() for x in ('q', 'k', 'v', 'grad_out')}
+    for i, n in enumerate([150, 0, 65, 130]):
+        for j, x in enumerate(dirty):
+            dirty[x][i, n:] = (float('nan'), float('inf'))[(i + j) % 2]
+    lengths = torch.tensor([1 << 40, -5, 65, 130], device='cuda')
+    args = [dirty['q'], dirty['k'], dirty['v'], p['log_decay'], lengths, p['initial_state']]
+    got = ops.decay_attention(*args, return_state=True) + ops.decay_attention_backward(dirty['grad_out'], *args, grad_state=p['grad_state'])
+    for x, y in zip(got, want):
+        assert torch.equal(x, y)
+    assert torch.equal(got[1][1], p['initial_state'][1]) and torch.equal(got[6][1], p['grad_state'][1])       # nothing happened there
+
+
+@gpu
+def test_decay_attention_is_causal_for_values_that_are_no_numbers():
+    """a NaN at one step leaves every result before it as it was"""
+    p = to_gpu(problem(1, 200, 1, 16, 16, 'f32', seed=5))
+    want = ops.decay_attention(p['q'], p['k'], p['v'], p['log_decay'])
+    for name in ('k', 'v', 'q'):
+        bad = dict(p)
+        bad[name] = p[name].clone()
+        bad[name][0, 101, 0, 3] = float('nan')
+        got = ops.decay_attention(bad['q'], bad['k'], bad['v'], p['log_decay'])
+        assert torch.equal(got[0, :101], want[0, :101]) and torch.isnan(got[0, 101]).any()
+
+
+@gpu
+def test_decay_attention_extreme_decays():
+    """no memory at all (-inf), no decay (0), a decay that underflows within a few steps"""
+    p = problem(2, 190, 3, 16, 16, 'f32', ragged=True, state=True, seed=6)
+    p['log_decay'] = torch.tensor([-math.inf, 0.0, -40.0])
+    d = to_gpu(p)
+    got = ops.decay_attention(**{x: d[x] for x in ARGS}, return_state=True)
+    want = recurrence(*[to_f64(p)[x] for x in ARGS])
+    size = recurrence(*[to_f64(absolute(p))[x] for x in ARGS])
+    for x, y, z in zip(got, want, size):
+        assert_near(x, y, z, 190)
+    grads = ops.decay_attention_backward(d['grad_out'], *[d[x] for x in ARGS], grad_state=d['grad_state'])
+    assert all(torch.isfinite(x).all() for x in grads) and grads[3][0] == 0
+    p['log_decay'] = torch.tensor([-200.0, 0.0, -40.0])            # exp(-200) is 0 in 32 bits; its gradients are finite in 64
+    check_gradients(dict(zip(LEAVES, grads)), p, (2, 190, 3, 16, 16))
+
+
+@gpu
+def test_decay_attention_empty_and_long():
+    for b, t in ((0, 5), (2, 0)):
+        p = to_gpu(problem(max(b, 1), max(t, 1), 2, 8, 8, 'f32', state=True))
+        cut = {x: (p[x][:b] if p[x] is not None and x != 'log_decay' else p[x]) for x in p}
+        cut.update({x: cut[x][:, :t] for x in ('q', 'k', 'v', 'grad_out')})
+        out, state = ops.decay_attention(**{x: cut[x] for x in ARGS}, return_state=True)
+        assert out.shape == (b, t, 2, 8) and torch.equal(state, cut['initial_state'])
+        grads = ops.decay_attention_backward(cut['grad_out'], *[cut[x] for x in ARGS], grad_state=cut['grad_state'])
+        assert torch.equal(grads[4], cut['grad_state']) and (grads[3] == 0).all()
+    # one long row, and its continuation from a state is the same row
+    p = to_gpu(problem(1, 9001, 2, 16, 16, 'f32', state=True, seed=8))
+    whole, state = ops.decay_attention(**{x: p[x] for x in ARGS}, return_state=True)
+    cpu = problem(1, 9001, 2, 16, 16, 'f32', state=True, seed=8)
+    want = recurrence(*[to_f64(cpu)[x] for x in ARGS])
+    size = recurrence(*[to_f64(absolute(cpu))[x] for x in ARGS])
+    assert_near(whole, want[0], size[0], 9001)
+    assert_near(state, want[1], size[1], 9001)
+    cut = 4321
+    first, middle = ops.decay_attention(p['q'][:, :cut], p['k'][:, :cut], p['v'][:, :cut], p['log_decay'], None, p['initial_state'], True)
+    second, last = ops.decay_attention(p['q'][:, cut:], p['k'][:, cut:], p['v'][:, cut:], p['log_decay'], None, middle, True)
+    assert_near(torch.cat([first, second], 1), want[0], size[0], 9001)
+    assert_near(last, want[1], size[1], 9001)
+    got = dict(zip(LEAVES, ops.decay_attention_backward(p['grad_out'], *[p[x] for x in ARGS], grad_state=p['grad_state'])))
+    check_gradients(got, cpu, (1, 9001, 2, 16, 16))
+
+
+# ---- one step ---------------------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize('dtype', sorted(TYPES))
+@pytest.mark.parametrize('shape', [(1, 1, 16, 16), (5, 4, 64, 64), (3, 2, 7, 13), (2, 3, 128, 128), (70, 2, 48, 40), (2, 1, 1, 1),
+                                   (4, 2, 33, 100)], ids=str)
+def test_decay_attention_step(shape, dtype):
+    b, h, dk, dv = shape
+    p = problem(b, 1, h, dk, dv, dtype, state=True, seed=9)
+    d = to_gpu(p)
+    state = d['initial_state'].clone()
+    active = torch.arange(b, device='cuda') % 3 != 1
+    out = ops.decay_attention_step(d['q'][:, 0], d['k'][:, 0], d['v'][:, 0], d['log_decay'], state, active=active)
+    want, want_state = recurrence(*[to_f64(p)[x] for x in ARGS])
+    size, size_state = recurrence(*[to_f64(absolute(p))[x] for x in ARGS])
+    on = active.cpu()
+    assert_near(out[active], want[:, 0][on], size[:, 0][on], 1)
+    assert_near(state[active], want_state[on], size_state[on], 1)
+    assert (out[~active] == 0).all() and torch.equal(state[~active], d['initial_state'][~active])
+
+
+@gpu
+def test_steps_are_the_sequence():
+    p = to_gpu(problem(3, 90, 2, 32, 48, 'f32', state=True, seed=10))
+    state, rows = p['initial_state'].clone(), []
+    for i in range(90):
+        rows.append(ops.decay_attention_step(p['q'][:, i], p['k'][:, i], p['v'][:, i], p['log_decay'], state))
+    out, final = ops.decay_attention(**{x: p[x] for x in ARGS}, return_state=True)
+    cpu = problem(3, 90, 2, 32, 48, 'f32', state=True, seed=10)
+    size = recurrence(*[to_f64(absolute(cpu))[x] for x in ARGS])
+    assert_near(torch.stack(rows, 1), out.double().cpu(), 2 * size[0], 90)
+    assert_near(state, final.double().cpu(), 2 * size[1], 90)
+
+
+# ---- a teacher's top logits ---------------------------------------------------------------------------------------------
+def top_statement(x, k, temperature):
+    indices = np.stack([sorted(range(x.shape[1]), key=lambda v: (not math.isnan(row[v]), -row[v] if not math.isnan(row[v]) else 0, v))[:k]
+                        for row in x])
+    rest = np.empty(len(x))
+    for i, row in enumerate(x):
+        left = np.delete(row, indices[i])
+        most = left.max() if len(left) else -math.inf
+        rest[i] = most if math.isinf(most) else most / temperature + math.log(np.exp((left - most) / temperature).sum())
+    return np.take_along_axis(x, indices, 1), indices, rest
+
+
+@gpu
+@pytest.mark.parametrize('dtype', sorted(TYPES))
+@pytest.mark.parametrize('rows,classes,k', [(1, 1, 1), (7, 5, 3), (4, 5, 5), (3, 128, 128), (3, 129, 128), (5, 257, 4), (2, 1000, 100),
+                                            (3, 5003, 31), (2, 20011, 128), (1, 70001, 64)])
+def test_top_logits(rows, classes, k, dtype):
+    g = torch.Generator().manual_seed(classes + k)
+    x = (torch.randn(rows, classes, generator=g) * 3).to(TYPES[dtype])
+    x[-1] = torch.randint(0, 3, (classes,), generator=g).to(TYPES[dtype])            # ties everywhere
+    check_top(x, k, 2.0)
+
+
+def check_top(x, k, temperature):
+    t = ops.top_logits(x.cuda(), k, temperature)
+    values, indices, rest = top_statement(x.double().numpy(), k, temperature)
+    assert t.values.dtype == x.dtype and t.indices.dtype == torch.int32 and t.rest.dtype == torch.float32
+    assert np.array_equal(t.indices.cpu().numpy(), indices)
+    assert np.array_equal(t.values.double().cpu().numpy(), values, equal_nan=True)
+    got = t.rest.double().cpu().numpy()
+    fine = np.isfinite(rest)
+    assert np.array_equal(got[~fine], rest[~fine], equal_nan=True)
+    # each exponential errs by 4 roundings and its exponent's own, of at most 2^-24 of |x|; the sum by its depth; the result by half a step
+    tol = 2.0 ** -24 * (np.abs(rest[fine]) + 64 + 2 * np.abs(np.nan_to_num(x.double().numpy(), posinf=0, neginf=0)).max() / temperature)
+    off = np.abs(got[fine] - rest[fine])
+    assert (off <= tol).all(), off.max()
+
+
+@gpu
+def test_top_logits_strange_rows():
+    inf, nan = math.inf, math.nan
+    x = torch.zeros(9, 300)
+    x[0] = -inf
+    x[1, 5:] = -inf
+    x[2, 7] = inf
+    x[3, 100:110] = inf
+    x[4, 200] = nan
+    x[5] = torch.arange(300.0)
+    x[6] = -torch.arange(300.0)
+    x[7, ::2] = -0.0
+    x[8] = torch.finfo(torch.float32).min
+    for k in (1, 4, 8, 128):
+        check_top(x, k, 1.0)
+    # a row of one value, longer than any buffer; a row whose largest lie behind one another
+    check_top(torch.ones(2, 40000), 128, 1.0)
+    check_top(torch.arange(40000.0).repeat(2, 1), 128, 1.0)
+    check_top((torch.arange(40000) // 64 % 7).float().repeat(2, 1), 100, 1.0)
+    # rows of a wider tensor, not aligned
+    wide = torch.randn(6, 1001)
+    t, u = ops.top_logits(wide.cuda()[:, 1:], 10), ops.top_logits(wide[:, 1:].contiguous().cuda(), 10)
+    assert torch.equal(t.indices, u.indices) and torch.equal(t.rest, u.rest)
+    assert len(ops.top_logits(torch.empty(0, 7, device='cuda'), 3)) == 0
+
+
+# ---- the distillation loss ----------------------------------------------------------------------------------------------
+def distill_statement(x, values, indices, rest, temperature, weight=None):
+    """(row losses, gradient of their sum), 64 bits, one row after the other"""
+    n, classes = x.shape
+    loss, grad, size = np.zeros(n), np.zeros_like(x), np.zeros(n)
+    for r in range(n):
+        w = 1.0 if weight is None else weight[r]
+        at = {}
+        t = [(v / temperature, i) for v, i in zip(values[r], indices[r]) if i != -1]
+        tail = -math.inf if rest is None else rest[r]
+        most = max([v for v, _ in t] + [tail])
+        if w == 0 or most == -math.inf:
+            continue
+        total = sum(math.exp(v - most) for v, _ in t) + math.exp(tail - most)
+        for v, i in t:
+            at[i] = at.get(i, 0.0) + math.exp(v - most) / total
+        pr = math.exp(tail - most) / total
+        y = x[r] / temperature
+        z = y.max() + math.log(np.exp(y - y.max()).sum())
+        q = np.exp(y - z)
+        off = np.ones(classes, bool)
+        off[list(at)] = False
+        qr = q[off].sum()
+        terms = [p * (math.log(p) - (y[i] - z)) for i, p in at.items() if p > 0] + ([pr * (math.log(pr) - math.log(qr))] if pr > 0 else [])
+        loss[r] = w * temperature ** 2 * sum(terms)
+        g = q.copy()
+        if pr > 0:
+            g[off] -= pr * q[off] / qr
+        for i, p in at.items():
+            g[i] -= p
+        grad[r] = w * temperature * g
+        # what float32 puts in: the largest exponent's rounding in each share
+        size[r] = w * temperature ** 2 * (1 + np.abs(y[np.isfinite(y)] - y.max()).max())
+    return loss, grad, size
+
+
+def distill_problem(rows, classes, k, dtype, temperature, seed=0):
+    g = torch.Generator().manual_seed(classes * 3 + k + seed)
+    teacher = torch.randn(rows, classes, generator=g) * 3
+    x = (teacher + torch.randn(rows, classes, generator=g)).to(TYPES[dtype])
+    values, indices, rest = top_statement(teacher.to(TYPES[dtype]).double().numpy(), k, temperature)
+    weight = torch.rand(rows, generator=g)
+    weight[rows // 2] = 0.0
+    return x, ops.TopLogits(torch.from_numpy(values).to(TYPES[dtype]), torch.from_numpy(indices).int(), torch.from_numpy(rest).float(),
+                            temperature), weight
+
+
+def check_distill(x, teacher, weight, reduction='none', grad_loss=None):
+    rows = len(x)
+    d, w = x.cuda().requires_grad_(), None if weight is None else weight.cuda()
+    t = teacher.to('cuda')
+    loss = ops.distillation_loss(d, t, w, reduction)
+    g = torch.linspace(0.5, 1.5, rows) if reduction == 'none' else torch.tensor(1.25)
+    grad = torch.autograd.grad(loss, d, g.cuda())[0]
+    both = ops.distillation_loss_and_gradient(d, t, w, reduction, g.cuda())
+    assert torch.equal(both[0], loss.detach()) and torch.equal(both[1], grad)
+    want, want_grad, size = distill_statement(x.double().numpy(), teacher.values.double().numpy(), teacher.indices.numpy(),
+                                              None if teacher.rest is None else teacher.rest.double().numpy(), teacher.temperature,
+                                              None if weight is None else weight.double().numpy())
+    scale = g.double().numpy() if reduction == 'none' else np.full(rows, float(g) / (rows if reduction == 'mean' else 1))
+    want_grad = want_grad * scale[:, None]
+    if reduction != 'none':
+        want, size = want.sum() / (rows if reduction == 'mean' else 1), size.sum() / (rows if reduction == 'mean' else 1)
+    # a share errs by the roundings of an exponential (its exponent's are in `size`) and of a sum over the classes
+    assert loss.dtype == torch.float32 and grad.dtype == x.dtype
+    off = np.abs(loss.detach().double().cpu().numpy() - want)
+    assert (off <= 2.0 ** -24 * (np.abs(want) + 64 * size)).all(), (off.max(), np.max(size))
+    room = (np.abs(scale) * (1.0 if weight is None else weight.double().numpy()) * teacher.temperature)[:, None]
+    per = 2.0 ** -24 * 64 * (1 + np.abs(np.nan_to_num(x.double().numpy(), neginf=0.0)).max(1, keepdims=True) / teacher.temperature) * room
+    q = torch.softmax(x.double() / teacher.temperature, 1).numpy()
+    # an unlisted class's gradient is a multiple of its share; a listed one's a difference of two shares
+    bound = per * np.maximum(q, np.where(np.abs(want_grad) > 0, 2.0 ** -24, 0))
+    for r in range(rows):
+        bound[r, teacher.indices[r].clamp(min=0).numpy()] = per[r]
+    if x.dtype == torch.float16:
+        bound = bound + 2.0 ** -25
+    tol = torch.finfo(x.dtype).eps / 2 * np.abs(want_grad) + bound + 1e-37
+    off = np.abs(grad.double().cpu().numpy() - want_grad)
+    assert (off <= tol * (1 + 2.0 ** -7)).all(), ((off - tol).max(), off.max())
+    return loss, grad
+
+
+@gpu
+@pytest.mark.parametrize('dtype', sorted(TYPES))
+@pytest.mark.parametrize('rows,classes,k,temperature', [(1, 1, 1, 1.0), (6, 5, 3, 2.0), (5, 5, 5, 1.5), (4, 300, 1, 1.0), (3, 257, 128, 4.0),
+                                                        (3, 2048, 17, 1.0), (5, 5001, 100, 4.0), (2, 40003, 64, 1.0)])
+def test_distillation_loss(rows, classes, k, temperature, dtype):
+    x, teacher, weight = distill_problem(rows, classes, k, dtype, temperature)
+    for reduction in ('none', 'mean', 'sum'):
+        check_distill(x, teacher, weight, reduction)
+    check_distill(x, teacher, None)
+    check_distill(x, ops.TopLogits(teacher.values, teacher.indices.long(), None, temperature), weight)
+
+
+@gpu
+def test_distillation_loss_against_differences():
+    """of the operator's own loss: an error of the loss's rounding over the step, and a step's square times the third derivative,
+    which is below w / temperature^3 * temperature^2 per unit of the direction's cube"""
+    x, teacher, weight = distill_problem(4, 200, 9, 'f32', 2.0, seed=1)
+    t, w = teacher.to('cuda'), weight.cuda()
+    loss, grad = ops.distillation_loss_and_gradient(x.cuda(), t, w, 'sum')
+    g = torch.Generator().manual_seed(2)
+    for _ in range(3):
+        d = torch.randn(x.shape, generator=g).cuda()
+        e = 2.0 ** -6
+        up, down = (ops.distillation_loss(x.cuda() + s * e * d, t, w, 'sum').double() for s in (1, -1))
+        want = float((grad.double() * d.double()).sum())
+        room = 64 * 16 * 4 * float(weight.sum()) * 2.0 ** -24 / e + e * e * float(weight.sum()) * float(d.abs().max()) ** 3
+        assert abs(float(up - down) / (2 * e) - want) <= room
+
+
+@gpu
+def test_distillation_loss_strange_rows():
+    inf, nan = math.inf, math.nan
+    x, teacher, _ = distill_problem(12, 50, 6, 'f32', 1.0, seed=3)
+    v, i, r = teacher.values, teacher.indices, teacher.rest
+    i[1, 2:] = -1                                        # empty places
+    i[2] = -1                                            # nothing listed: the rest alone
+    i[3, 4] = i[3, 1]                                    # a class twice
+    i[4] = i[4, 0]                                       # one class in every place
+    v[5, 3:] = -inf                                      # places without a share
+    r[6] = -inf                                          # nothing unlisted
+    i[7], r[7] = -1, -inf                                # nothing at all
+    x[8, i[8, 5].item()] -= 200.0                        # far below, but a number
+    x[9, [c for c in range(50) if c not in i[9].tolist()]] = -150.0           # the unlisted far below the listed
+    weight = torch.ones(12)
+    weight[10] = 0.0
+    x[10] = nan                                          # a row that does not count may hold anything
+    x[11, [c for c in range(50) if c not in i[11].tolist()][3]] = -inf        # one class ruled out
+    rows = list(range(12))
+    rows.remove(10)
+    loss, grad = check_distill(x[rows], teacher[rows], None)
+    assert float(loss[7].detach()) == 0 and (grad[7] == 0).all()
+    loss, grad = ops.distillation_loss_and_gradient(x.cuda(), teacher.to('cuda'), weight.cuda(), 'none')
+    assert float(loss[10]) == 0 and (grad[10] == 0).all() and torch.isfinite(loss).all() and torch.isfinite(grad).all()
+    # a share where the student has none: infinite, with finite gradients; what is no class: NaN in its row alone
+    x, teacher, _ = distill_problem(4, 50, 6, 'f32', 1.0, seed=4)
+    x[1, int(teacher.indices[1, 0])] = -inf
+    teacher.indices[2, 1], teacher.indices[3, 0] = 50, -2
+    loss, grad = ops.distillation_loss_and_gradient(x.cuda(), teacher.to('cuda'), None, 'none')
+    assert math.isinf(loss[1]) and torch.isfinite(grad[:2]).all() and torch.isfinite(loss[0])
+    assert torch.isnan(loss[2:]).all() and torch.isnan(grad[2:]).all()
+    assert torch.isnan(ops.distillation_loss(x.cuda(), teacher.to('cuda')))
+    empty = ops.TopLogits(torch.empty(0, 3, device='cuda'), torch.empty(0, 3, dtype=torch.int32, device='cuda'))
+    none = torch.empty(0, 9, device='cuda', requires_grad=True)
+    assert float(ops.distillation_loss(none, empty, reduction='sum')) == 0
+
+
+# ---- together, streams, graphs ----------------------------------------------------------------------------------------------
+@gpu
+def test_teacher_student_together():
+    """a layer's result through a linear map is the student, another map the teacher: one step's loss and gradients"""
+    g = torch.Generator().manual_seed(11)
+    b, t, h, d, classes, k, tau = 6, 70, 2, 16, 37, 5, 2.0
+    p = problem(b, t, h, d, d, 'f32', ragged=True, seed=11)
+    p['lengths'][1] = 3
+    head, teach = torch.randn(h * d, classes, generator=g) * 0.3, torch.randn(b * t, classes, generator=g) * 2
+    weight = (torch.arange(t) < p['lengths'][:, None]).float().flatten()
+    teacher = ops.top_logits(teach.cuda(), k, tau)
+    leaf = [p[x].cuda().requires_grad_() for x in ('q', 'k', 'v', 'log_decay')] + [head.cuda().requires_grad_()]
+    out = ops.decay_attention(*leaf[:4], lengths=p['lengths'].cuda())
+    loss = ops.distillation_loss(out.reshape(b * t, h * d) @ leaf[4], teacher, weight.cuda())
+    got = torch.autograd.grad(loss, leaf)
+    plain = [x.detach().double().cpu().requires_grad_() for x in leaf]
+    o, _ = recurrence(*plain[:4], p['lengths'])
+    y = o.reshape(b * t, h * d) @ plain[4] / tau
+    values, indices, rest = top_statement(teach.double().numpy(), k, tau)
+    both = torch.log_softmax(torch.cat([torch.from_numpy(values) / tau, torch.from_numpy(rest)[:, None]], 1), 1)
+    z, index = torch.log_softmax(y, 1), torch.from_numpy(indices)
+    away = torch.ones_like(z, dtype=torch.bool).scatter_(1, index, False)
+    logq = torch.cat([z.gather(1, index), z.masked_fill(~away, -math.inf).logsumexp(1, keepdim=True)], 1)
+    want_loss = (weight.double() * (both.exp() * (both - logq)).sum(1)).mean() * tau ** 2
+    want = torch.autograd.grad(want_loss, plain)
+    # a float32 product of 32 terms and sums of up to 420 rows on the way: 1e-5 of the gradient's norm is 2^-24 * 168
+    assert abs(loss.item() - want_loss.item()) <= 1e-5 * abs(want_loss.item())
+    for x, y in zip(got, want):
+        assert float((x.double().cpu() - y).norm()) <= 1e-5 * float(y.norm())
+
+
+@gpu
+def test_streams_and_graphs():
+    """another stream than the tensors' own; every call captured (two graphs, alive together) and replayed several times with
+    eager work between, new inputs each time"""
+    p = to_gpu(problem(2, 200, 2, 32, 32, 'bf16', True, True, seed=12))
+    x, teacher, weight = distill_problem(33, 700, 9, 'f32', 2.0, seed=12)
+    x, teacher, weight = x.cuda(), teacher.to('cuda'), weight.cuda()
+    args = [p[n] for n in ARGS]
+    state = p['initial_state'].clone()
+
+    def everything():
+        outs = list(ops.decay_attention(*args, return_state=True))
+        outs += ops.decay_attention_backward(p['grad_out'], *args, grad_state=p['grad_state'])
+        outs.append(ops.decay_attention_step(p['q'][:, 0], p['k'][:, 0], p['v'][:, 0], p['log_decay'], state))
+        t = ops.top_logits(x, 9, 2.0)
+        outs += [t.values, t.indices, t.rest, *ops.distillation_loss_and_gradient(x, teacher, weight)]
+        return outs + [state]
+    first = state.clone()
+    want = [y.clone() for y in everything()]
+    state.copy_(first)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = [y.clone() for y in everything()]
+    torch.cuda.current_stream().wait_stream(side)
+    for y, z in zip(got, want):
+        assert torch.equal(y, z)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = everything()
+        graphs.append((graph, outs))
+    for turn in range(4):
+        p['q'].mul_(0.5), x.add_(torch.randn_like(x))
+        state.copy_(first)
+        want = [y.clone() for y in everything()]
+        for graph, outs in graphs:
+            state.copy_(first)
+            graph.replay()
+            torch.cuda.synchronize()
+            for y, z in zip(outs, want):
+                assert torch.equal(y, z), turn
+
+
+@gpu
+def test_captured_backward_beside_an_eager_graph():
+    """Refused before anything happens: the backward pass would have to wait, inside the capture, for the stream of the eager
+    graph.  With that graph gone the same capture works."""
+    p = to_gpu(problem(1, 20, 1, 8, 8, 'f32', seed=13))
+    q = p['q'].requires_grad_()
+    eager = ops.decay_attention(q, p['k'], p['v'], p['log_decay'])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='alive'):
+        with torch.cuda.graph(graph):
+            ops.decay_attention(q, p['k'], p['v'], p['log_decay'])
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(eager, q, p['grad_out'])[0]
+    del eager, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(ops.decay_attention(q, p['k'], p['v'], p['log_decay']), q, p['grad_out'])[0]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+# ---- refusals (on the CPU: nothing is launched) -------------------------------------------------------------------------
+@pytest.fixture
+def dry(monkeypatch):
+    """the checks of arguments alone: CPU tensors pass as GPU tensors, a launch fails the test"""
+    monkeypatch.setattr(ops, '_on_gpu', lambda name, t, device=None: None)
+
+    def launched(*a):
+        raise AssertionError('launched')
+    monkeypatch.setattr(ops, '_call', launched)
+    monkeypatch.setattr(ops, '_lib', launched)
+    monkeypatch.setattr(ops, '_differentiable', launched)
+
+
+def test_cpu_tensors_are_refused():
+    p = problem(1, 4, 1, 8, 8, 'f32')
+    with pytest.raises(ValueError, match='on a GPU only'):
+        ops.decay_attention(*[p[x] for x in ARGS[:4]])
+    with pytest.raises(ValueError, match='on a GPU only'):
+        ops.top_logits(torch.zeros(2, 3), 1)
+    with pytest.raises(ValueError, match='on a GPU only'):
+        ops.distillation_loss(torch.zeros(2, 3), ops.TopLogits(torch.zeros(2, 1), torch.zeros(2, 1, dtype=torch.int32)))
+    with pytest.raises(TypeError, match='must be a tensor'):
+        ops.top_logits([[1.0]], 1)
+
+
+def test_decay_refusals(dry):
+    p = problem(2, 4, 3, 8, 6, 'f32', state=True)
+    args = {x: p[x] for x in ARGS}
+    for change, error, text in [
+            ({'k': p['k'].bfloat16()}, TypeError, 'k is'), ({'q': p['q'].double()}, TypeError, 'float32, bfloat16 or float16'),
+            ({'q': p['q'][0]}, ValueError, 'q, k and v'), ({'k': p['k'][..., :7]}, ValueError, 'q, k and v'),
+            ({'v': p['v'][:, :3]}, ValueError, 'q, k and v'), ({'v': p['v'][:, :, :2]}, ValueError, 'q, k and v'),
+            ({'v': torch.zeros(2, 4, 3, 129)}, ValueError, 'widths'), ({'v': torch.zeros(2, 4, 3, 0)}, ValueError, 'widths'),
+            ({'log_decay': p['log_decay'][:2]}, ValueError, 'log_decay'), ({'log_decay': p['log_decay'].double()}, TypeError, 'log_decay'),
+            ({'lengths': torch.ones(2)}, TypeError, 'lengths'), ({'lengths': torch.ones(3, dtype=torch.int32)}, ValueError, 'lengths'),
+            ({'initial_state': p['initial_state'].half()}, TypeError, 'initial_state'),
+            ({'initial_state': p['initial_state'].transpose(2, 3)}, ValueError, 'initial_state')]:
+        with pytest.raises(error, match=text):
+            ops.decay_attention(**{**args, **change})
+    with pytest.raises(ValueError, match='grad_out'):
+        ops.decay_attention_backward(p['grad_out'][:, :3], **args)
+    with pytest.raises(ValueError, match='grad_state'):
+        ops.decay_attention_backward(p['grad_out'], **args, grad_state=p['grad_state'][:1])
+    one = {x: p[x][:, 0] for x in ('q', 'k', 'v')}
+    step = {**one, 'log_decay': p['log_decay'], 'state': p['initial_state']}
+    for change, error, text in [({'q': p['q']}, ValueError, 'q, k and v'), ({'state': p['initial_state'][:1]}, ValueError, 'state'),
+                                ({'state': p['initial_state'].transpose(2, 3).contiguous().transpose(2, 3)}, ValueError, 'contiguous'),
+                                ({'active': torch.ones(2)}, ValueError, 'active'), ({'active': torch.ones(3).bool()}, ValueError, 'active'),
+                                ({'q': one['q'].clone().requires_grad_()}, RuntimeError, 'no gradients')]:
+        with pytest.raises(error, match=text):
+            ops.decay_attention_step(**{**step, **change})
+
+
+def test_distillation_refusals(dry):
+    x = torch.zeros(4, 9)
+    good = ops.TopLogits(torch.zeros(4, 3), torch.zeros(4, 3, dtype=torch.int32), torch.zeros(4), 2.0)
+    for logits, k, temperature, error, text in [
+            (x.double(), 2, 1.0, TypeError, 'float32'), (x[0], 2, 1.0, ValueError, 'rows, classes'), (x, 0, 1.0, ValueError, 'k is'),
+            (x, 10, 1.0, ValueError, 'k is'), (torch.zeros(2, 200), 129, 1.0, ValueError, 'k is'), (x, 2, 0.0, ValueError, 'temperature'),
+            (x, 2, float('nan'), ValueError, 'temperature'), (x, 2, float('inf'), ValueError, 'temperature'),
+            (torch.zeros(4, 0), 1, 1.0, ValueError, 'rows, classes')]:
+        with pytest.raises(error, match=text):
+            ops.top_logits(logits, k, temperature)
+    t = good
+    for logits, teacher, options, error, text in [
+            (x.double(), t, {}, TypeError, 'float32'), (x, (t.values, t.indices), {}, TypeError, 'TopLogits'),
+            (x[:3], t, {}, ValueError, 'teacher.values'), (x, ops.TopLogits(t.values, t.indices.float(), t.rest), {}, TypeError, 'indices'),
+            (x, ops.TopLogits(t.values, t.indices[:, :2], t.rest), {}, ValueError, 'teacher.values'),
+            (x, ops.TopLogits(t.values, t.indices, t.rest.double()), {}, TypeError, 'rest'),
+            (x, ops.TopLogits(t.values, t.indices, t.rest[:2]), {}, ValueError, 'rest'),
+            (x, ops.TopLogits(t.values, t.indices, t.rest, -1.0), {}, ValueError, 'temperature'),
+            (x, ops.TopLogits(torch.zeros(4, 129), torch.zeros(4, 129).int(), t.rest), {}, ValueError, 'up to 128'),
+            (x, t, {'weight': torch.zeros(3)}, ValueError, 'weight'), (x, t, {'weight': torch.zeros(4).half()}, TypeError, 'weight'),
+            (x, t, {'weight': torch.zeros(4, requires_grad=True)}, ValueError, 'gradient'),
+            (x, t, {'reduction': 'avg'}, ValueError, 'reduction')]:
+        with pytest.raises(error, match=text):
+            ops.distillation_loss(logits, teacher, **options)
+    with pytest.raises(ValueError, match='grad_loss'):
+        ops.distillation_loss_and_gradient(x, t, grad_loss=torch.zeros(4))
+
+
+def test_top_logits_rows():
+    t = ops.TopLogits(torch.arange(8.0).view(4, 2), torch.arange(8).view(4, 2), torch.arange(4.0), 2.0)
+    assert len(t) == 4 and t[torch.tensor([2, 0])].rest.tolist() == [2.0, 0.0] and t[1].values.tolist() == [[2.0, 3.0]]
+    assert t[-1].indices.tolist() == [[6, 7]] and t.to('cpu').temperature == 2.0 and t[1:3].temperature == 2.0
+    both = ops.TopLogits.cat([t[:1], t[1:]])
+    assert both.values.equal(t.values) and both.rest.equal(t.rest)
+    with pytest.raises(ValueError, match='temperatures'):
+        ops.TopLogits.cat([t, ops.TopLogits(t.values, t.indices, t.rest, 1.0)])
+    assert ops.TopLogits(t.values, t.indices)[0].rest is None
+
+
+def test_c_entries_refuse_what_they_can_see():
+    """bad shapes, types and missing pointers come back as PXG_E_INVALID before anything touches a GPU"""
+    lib = N.load_library()
+    invalid = -1
+    s = N.PxgDecay()
+    assert lib.pxg_decay_forward(C.byref(s), None) == invalid                     # struct_bytes
+    s.struct_bytes, s.batch, s.steps, s.heads, s.dk, s.dv = C.sizeof(s), 1, 1, 1, 8, 8
+    for fn in (lib.pxg_decay_forward, lib.pxg_decay_backward, lib.pxg_decay_step):
+        assert fn(C.byref(s), None) == invalid and fn(None, None) == invalid      # no pointers
+    for field, value in (('dtype', 3), ('dk', 129), ('dk', 0), ('dv', -1), ('heads', 0), ('batch', -1), ('steps', -1),
+                         ('batch', 1 << 40), ('steps', 1 << 40)):
+        t = N.PxgDecay.from_buffer_copy(s)
+        setattr(t, field, value)
+        assert lib.pxg_decay_workspace_bytes(C.byref(t), 1) == invalid, field
+    t = N.PxgDecay.from_buffer_copy(s)
+    t.batch, t.log_decay = 0, 4096
+    assert lib.pxg_decay_forward(C.byref(t), None) == 0                           # nothing to do
+    d = N.PxgDistill()
+    assert lib.pxg_distill_forward(C.byref(d), None) == invalid
+    d.struct_bytes, d.rows, d.classes, d.temperature, d.k = C.sizeof(d), 1, 8, 1.0, 2
+    assert lib.pxg_distill_forward(C.byref(d), None) == invalid and lib.pxg_distill_backward(C.byref(d), None) == invalid
+    d.rows = 0
+    assert lib.pxg_distill_forward(C.byref(d), None) == 0 and lib.pxg_distill_backward(C.byref(d), None) == 0
+    for field, value in (('k', 129), ('k', -1), ('classes', 0), ('temperature', 0.0), ('temperature', float('nan')), ('dtype', -1),
+                         ('value_dtype', 7)):
+        e = N.PxgDistill.from_buffer_copy(d)
+        setattr(e, field, value)
+        assert lib.pxg_distill_forward(C.byref(e), None) == invalid, field
+    top = lambda dt=0, rows=1, classes=8, k=2, tau=1.0: lib.pxg_top_logits(dt, rows, classes, None, 8, k, tau, None, None, None, None)  # noqa: E731
+    assert top() == top(rows=-1) == top(k=0) == top(k=9) == top(tau=0.0) == top(dt=5) == invalid and top(rows=0) == 0
+
+
+def test_structs_match_the_header():
+    import os
+    import subprocess
+    import tempfile
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    src = '#include <stdio.h>\n#include "pxg.h"\nint main(){printf("%zu %zu %zu", sizeof(pxg_sequence), sizeof(pxg_decay), sizeof(pxg_distill));return 0;}'
+    with tempfile.TemporaryDirectory() as d:
+        open(os.path.join(d, 'sz.c'), 'w').write(src)
+        exe = os.path.join(d, 'sz')
+        subprocess.check_call(['gcc', '-I' + os.path.join(root, 'include'), os.path.join(d, 'sz.c'), '-o', exe])
+        sizes = [int(v) for v in subprocess.check_output([exe]).split()]
+    assert sizes == [C.sizeof(N.PxgSequence), C.sizeof(N.PxgDecay), C.sizeof(N.PxgDistill)]
