@@ -1,0 +1,50 @@
+// k_decay.h -- what the sources of decay attention share: the operands of one run of the recurrence (k_decay.hip says which
+// four runs a training step consists of) and the launchers, one source for each element type.
+#pragma once
+#include "pxg_ops.h"
+
+struct DecayRun {
+    pxg_sequence x, y, z;      // operands: widths E, E, F
+    const float* init;         // state before the first step (of the run's direction), element (e, f) at e * init_e + f * init_f
+    float* fin;                // state behind the last one, same layout
+    int64_t init_e, init_f;
+    void* out;                 // [batch][steps][heads][F]
+    int E, F;
+    int reverse;               // steps taken from the last to the first; then init joins the first step without decay
+    int wide;                  // bits 0..3: rows of x, y, z, dot can be read 16 bytes at a time, bit 4: rows of out written 4 values at a time
+    float* carry;              // states between segments, [batch * heads][segments - 1][E][F] (and the slopes behind them)
+    // gradient of log_decay (the run of dq): q's rows, the gradient of the final state, one partial sum per (batch * heads, segment)
+    pxg_sequence dot;
+    const float* grad_fin;
+    float* partial;
+};
+
+struct DecayRuns {
+    DecayRun run[3];
+    int64_t steps;
+    int batch, heads;
+    const float* log_decay;
+    const void* lengths;
+    int lengths_are_64;
+    int segments, segment_chunks;      // the time axis in so many pieces of so many chunks, each a workgroup of its own
+};
+
+__device__ __forceinline__ int64_t decay_length(const DecayRuns& s, int b)
+{
+    if (!s.lengths) return s.steps;
+    const int64_t n = s.lengths_are_64 ? ((const int64_t*)s.lengths)[b] : (int64_t)((const int32_t*)s.lengths)[b];
+    return n < 0 ? 0 : n > s.steps ? s.steps : n;
+}
+
+// steps in a chunk, by the type's number of bfloat16 planes and the padded width
+constexpr int decay_chunk(int dtype, int width) { return dtype == PXG_DT_F32 && width > 32 ? 32 : 64; }
+constexpr int decay_width(int e, int f)
+{
+    const int w = e > f ? e : f;
+    return w <= 16 ? 16 : w <= 32 ? 32 : w <= 64 ? 64 : 128;
+}
+
+// `n` runs starting at run[first]; slope: the run carries dS/dlog_decay; states_only: nothing but `carry` is written
+int decay_launch_f32(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream);
+int decay_launch_bf16(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream);
+int decay_launch_f16(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream);

@@ -8,115 +8,40 @@
 //   dk = run(x v,  y do, z q) backwards               dv = run(x k,  y q,  z do) backwards  with R = dL/dS as their state
 // and the gradient of log_decay is sum_t do_t . (q_t D_t) + <dL/dS_T, D_T> with D = dS/dlog_decay = a (D + S) carried beside S
 // in the run of dq: no difference of large sums, however long the sequence.
-#include "pxg_ops.h"
+//
+// The runs themselves are in k_decay_chunk.h.
+#include "k_decay.h"
 
 namespace {
 
-struct DecayRun {
-    pxg_sequence x, y, z;      // operands: widths E, E, F
-    const float* init;         // state before the first step (of the run's direction), element (e, f) at e * init_e + f * init_f
-    float* fin;                // state behind the last one, same layout
-    int64_t init_e, init_f;
-    void* out;                 // [batch][steps][heads][F]
-    int E, F;
-    int reverse;               // steps taken from the last to the first; then init joins the first step without decay
-    // gradient of log_decay (the run of dq): q's rows, the gradient of the final state, one partial sum per (batch, head)
-    pxg_sequence dot;
-    const float* grad_fin;
-    float* partial;
-};
-
-struct DecayShape {
-    int64_t steps;
-    int batch, heads;
-    const float* log_decay;
-    const void* lengths;
-    int lengths_are_64;
-};
-
-__device__ __forceinline__ int64_t decay_length(const DecayShape& s, int b)
+// carry[s] becomes the state in front of segment s + 1: each segment's own, plus what came before it, decayed over its length;
+// the slopes behind the states decay and grow with the distance.
+__global__ __launch_bounds__(256) void k_decay_join(const DecayRuns a, int chunk, int slope_runs)
 {
-    if (!s.lengths) return s.steps;
-    const int64_t n = s.lengths_are_64 ? ((const int64_t*)s.lengths)[b] : (int64_t)((const int32_t*)s.lengths)[b];
-    return n < 0 ? 0 : n > s.steps ? s.steps : n;
-}
-
-// One step after the other, the state in shared memory: thread f owns column f.
-template <typename T, bool DER>
-__global__ __launch_bounds__(128) void k_decay_serial(DecayRun r, DecayShape s)
-{
-    extern __shared__ float lds[];
-    const int f = threadIdx.x, b = blockIdx.x / s.heads, h = blockIdx.x % s.heads;
-    float* S = lds;
-    float* D = S + r.E * r.F;
-    float* xs = D + (DER ? r.E * r.F : 0);
-    float* ys = xs + r.E;
-    const int64_t len = decay_length(s, b), base = (int64_t)blockIdx.x * r.E * r.F;
-    const float a = expf(s.log_decay[h]);
-    const T* x = (const T*)r.x.data + b * r.x.batch_stride + h * r.x.head_stride;
-    const T* y = (const T*)r.y.data + b * r.y.batch_stride + h * r.y.head_stride;
-    const T* z = (const T*)r.z.data + b * r.z.batch_stride + h * r.z.head_stride;
-    T* out = (T*)r.out + ((int64_t)b * s.steps * s.heads + h) * r.F;
-    const int64_t out_step = (int64_t)s.heads * r.F;
-    if (f < r.F)
-        for (int e = 0; e < r.E; e++) {
-            S[e * r.F + f] = r.init ? r.init[base + e * r.init_e + f * r.init_f] : 0.f;
-            if (DER) D[e * r.F + f] = 0.f;
-        }
-    float part = 0.f;
-    for (int64_t u = 0; u < len; u++) {
-        const int64_t t = r.reverse ? len - 1 - u : u;
-        for (int e = f; e < r.E; e += blockDim.x) {
-            xs[e] = pxg_to_f32(x[t * r.x.step_stride + e]);
-            ys[e] = pxg_to_f32(y[t * r.y.step_stride + e]);
-        }
-        __syncthreads();
-        if (f < r.F) {
-            const float zf = pxg_to_f32(z[t * r.z.step_stride + f]), decay = r.reverse && u == 0 ? 1.f : a;
-            float o = 0.f, d = 0.f;
-            for (int e = 0; e < r.E; e++) {
-                const float old = S[e * r.F + f], now = fmaf(decay, old, ys[e] * zf);
-                S[e * r.F + f] = now;
-                o = fmaf(xs[e], now, o);
-                if (DER) {
-                    const float dn = decay * (D[e * r.F + f] + old);
-                    D[e * r.F + f] = dn;
-                    d = fmaf(xs[e], dn, d);
-                }
-            }
-            out[t * out_step + f] = pxg_from_f32<T>(o);
-            if (DER) {
-                const T* q = (const T*)r.dot.data + b * r.dot.batch_stride + h * r.dot.head_stride;
-                part = fmaf(pxg_to_f32(q[t * r.dot.step_stride + f]), d, part);
-            }
-        }
-        __syncthreads();
-    }
-    if (f < r.F) {
-        for (int64_t t = len; t < s.steps; t++) out[t * out_step + f] = pxg_from_f32<T>(0.f);
-        for (int e = 0; e < r.E; e++) {
-            if (r.fin) r.fin[base + e * r.init_e + f * r.init_f] = r.reverse && len ? a * S[e * r.F + f] : S[e * r.F + f];
-            if (DER && r.grad_fin) part = fmaf(r.grad_fin[base + e * r.init_e + f * r.init_f], D[e * r.F + f], part);
-        }
-    }
-    if (DER) {
-        __syncthreads();
-        xs[f] = f < r.F ? part : 0.f;
-        __syncthreads();
-        if (f == 0) {
-            float sum = 0.f;
-            for (int i = 0; i < (int)blockDim.x; i++) sum += xs[i];
-            r.partial[blockIdx.x] = sum;
-        }
+    const DecayRun& r = a.run[blockIdx.z];
+    const int64_t size = (int64_t)r.E * r.F, bh = blockIdx.x, n = a.segments - 1;
+    const int64_t slopes = (int64_t)a.batch * a.heads * n * size;
+    const int i = blockIdx.y * 256 + threadIdx.x;
+    if (i >= size) return;
+    const int64_t len = decay_length(a, (int)(bh / a.heads)), used = (len + chunk - 1) / chunk;
+    const float steps = (float)a.segment_chunks * (float)chunk, decay = expf(steps * a.log_decay[bh % a.heads]);
+    const bool slope = (int)blockIdx.z < slope_runs;
+    float* c = r.carry + bh * n * size + i;
+    float S = c[0], G = slope ? c[slopes] : 0.f;
+    for (int64_t s = 1; s < n && (s + 1) * a.segment_chunks < used; s++) {
+        c += size;
+        if (slope) c[slopes] = G = fmaf(decay, G + steps * S, c[slopes]);
+        *c = S = fmaf(decay, S, *c);
     }
 }
 
-// grad_log_decay[h] = sum over the batch (and whatever else lies between) of the partial sums, in a fixed order
-__global__ __launch_bounds__(256) void k_decay_sum(const float* partial, int64_t n, int heads, float* out)
+// grad_log_decay[h] = the sum of the partial sums [batch][heads][segments], in a fixed order
+__global__ __launch_bounds__(256) void k_decay_sum(const float* partial, int64_t batch, int heads, int segments, float* out)
 {
     __shared__ double red[256];
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 256) sum += (double)partial[i * heads + blockIdx.x];
+    for (int64_t i = threadIdx.x; i < batch * segments; i += 256)
+        sum += (double)partial[(i / segments * heads + blockIdx.x) * segments + i % segments];
     red[threadIdx.x] = sum;
     __syncthreads();
     for (int w = 128; w; w >>= 1) {
@@ -126,24 +51,30 @@ __global__ __launch_bounds__(256) void k_decay_sum(const float* partial, int64_t
     if (threadIdx.x == 0) out[blockIdx.x] = (float)red[0];
 }
 
-template <typename T>
-int launch_run(const DecayRun& r, const DecayShape& s, hipStream_t stream)
-{
-    const size_t state = (size_t)r.E * r.F * sizeof(float), rows = (2 * (size_t)r.E + 128) * sizeof(float);
-    if (r.partial)
-        k_decay_serial<T, true><<<s.batch * s.heads, 128, 2 * state + rows, stream>>>(r, s);
-    else
-        k_decay_serial<T, false><<<s.batch * s.heads, 128, state + rows, stream>>>(r, s);
-    return hipGetLastError() == hipSuccess ? PXG_OK : PXG_E_HIP;
-}
-
-int run(const DecayRun& r, const DecayShape& s, int dtype, hipStream_t stream)
+int launch(const DecayRuns& a, int dtype, int first, int n, bool slope, bool states_only, hipStream_t stream)
 {
     switch (dtype) {
-    case PXG_DT_F32: return launch_run<float>(r, s, stream);
-    case PXG_DT_BF16: return launch_run<pxg_bf16>(r, s, stream);
-    default: return launch_run<pxg_f16>(r, s, stream);
+    case PXG_DT_F32: return decay_launch_f32(a, first, n, slope, states_only, stream);
+    case PXG_DT_BF16: return decay_launch_bf16(a, first, n, slope, states_only, stream);
+    default: return decay_launch_f16(a, first, n, slope, states_only, stream);
     }
+}
+
+// The first `slope_runs` of the `n` runs carry slopes.
+int launch_runs(const DecayRuns& a, int dtype, int n, int slope_runs, hipStream_t stream)
+{
+    int rc = PXG_OK;
+    if (a.segments > 1) {
+        if (slope_runs) rc = launch(a, dtype, 0, slope_runs, true, true, stream);
+        if (rc == PXG_OK && n > slope_runs) rc = launch(a, dtype, slope_runs, n - slope_runs, false, true, stream);
+        if (rc != PXG_OK) return rc;
+        const dim3 grid(a.batch * a.heads, (a.run[0].E * a.run[0].F + 255) / 256, n);
+        k_decay_join<<<grid, 256, 0, stream>>>(a, decay_chunk(dtype, decay_width(a.run[0].E, a.run[0].F)), slope_runs);
+        if (hipGetLastError() != hipSuccess) return PXG_E_HIP;
+    }
+    if (slope_runs) rc = launch(a, dtype, 0, slope_runs, true, false, stream);
+    if (rc == PXG_OK && n > slope_runs) rc = launch(a, dtype, slope_runs, n - slope_runs, false, false, stream);
+    return rc;
 }
 
 // One step: the state is read once and written once, which is all the time this takes.
@@ -185,10 +116,50 @@ bool bad_operands(const pxg_decay* a)
     return !a->log_decay || (any && (!a->q.data || !a->k.data || !a->v.data));
 }
 
-DecayShape shape_of(const pxg_decay* a)
+// How the time axis is cut: not at all where (sequence, head) pairs alone fill the card, else into enough segments that do, of at
+// least four chunks each.  What the segments cost is a second reading of y and z.
+struct Cut {
+    int segments, chunks;
+};
+
+Cut cut_of(const pxg_decay* a)
 {
-    DecayShape s = {a->steps, (int)a->batch, a->heads, a->log_decay, a->lengths, a->lengths_are_64};
+    const int64_t chunk = decay_chunk(a->dtype, decay_width(a->dk, a->dv)), chunks = (a->steps + chunk - 1) / chunk;
+    const int64_t pairs = a->batch * a->heads;
+    int64_t segments = pairs < 256 && pairs > 0 ? (512 + pairs - 1) / pairs : 1;
+    if (segments > chunks / 4) segments = chunks / 4;
+    if (segments < 1) segments = 1;
+    const int64_t each = segments > 1 ? (chunks + segments - 1) / segments : chunks > 0 ? chunks : 1;
+    Cut c = {(int)(segments > 1 ? (chunks + each - 1) / each : 1), (int)each};
+    return c;
+}
+
+int64_t carry_values(const pxg_decay* a, const Cut& c)
+{
+    return a->batch * a->heads * (c.segments - 1) * a->dk * a->dv;
+}
+
+DecayRuns runs_of(const pxg_decay* a, const Cut& c)
+{
+    DecayRuns s = {};
+    s.steps = a->steps, s.batch = (int)a->batch, s.heads = a->heads;
+    s.log_decay = a->log_decay, s.lengths = a->lengths, s.lengths_are_64 = a->lengths_are_64;
+    s.segments = c.segments, s.segment_chunks = c.chunks;
     return s;
+}
+
+// rows that can be read 16 bytes at a time, in whole groups of eight elements
+bool wide(const pxg_sequence& s, int width, int dtype)
+{
+    const int64_t unit = dtype == PXG_DT_F32 ? 4 : 8;
+    return (uintptr_t)s.data % 16 == 0 && width % 8 == 0 && s.batch_stride % unit == 0 && s.step_stride % unit == 0 &&
+           s.head_stride % unit == 0;
+}
+
+void finish_run(DecayRun& r, int dtype)
+{
+    r.wide = (wide(r.x, r.E, dtype) ? 1 : 0) | (wide(r.y, r.E, dtype) ? 2 : 0) | (wide(r.z, r.F, dtype) ? 4 : 0) |
+             ((uintptr_t)r.out % 16 == 0 && r.F % 4 == 0 ? 16 : 0);
 }
 
 }  // namespace
@@ -196,7 +167,9 @@ DecayShape shape_of(const pxg_decay* a)
 extern "C" int64_t pxg_decay_workspace_bytes(const pxg_decay* a, int32_t backward)
 {
     if (bad_shape(a)) return PXG_E_INVALID;
-    return backward ? a->batch * a->heads * (int64_t)sizeof(float) : 0;
+    const Cut c = cut_of(a);
+    // the states between segments (backward: of three runs, and the slopes of one), the partial sums of grad_log_decay
+    return (int64_t)sizeof(float) * (carry_values(a, c) * (backward ? 4 : 1) + (backward ? a->batch * a->heads * c.segments : 0));
 }
 
 extern "C" int pxg_decay_forward(const pxg_decay* a, void* stream)
@@ -204,11 +177,16 @@ extern "C" int pxg_decay_forward(const pxg_decay* a, void* stream)
     if (bad_shape(a) || bad_operands(a)) return PXG_E_INVALID;
     if (a->batch == 0) return PXG_OK;
     if (a->steps > 0 && !a->out) return PXG_E_INVALID;
-    DecayRun r = {};
+    const int64_t bytes = pxg_decay_workspace_bytes(a, 0);
+    if (a->workspace_bytes < bytes || (bytes > 0 && !a->workspace)) return PXG_E_INVALID;
+    DecayRuns s = runs_of(a, cut_of(a));
+    DecayRun& r = s.run[0];
     r.x = a->q, r.y = a->k, r.z = a->v;
     r.init = a->initial_state, r.fin = a->final_state, r.init_e = a->dv, r.init_f = 1;
     r.out = a->out, r.E = a->dk, r.F = a->dv;
-    return run(r, shape_of(a), a->dtype, (hipStream_t)stream);
+    r.carry = (float*)a->workspace;
+    finish_run(r, a->dtype);
+    return launch_runs(s, a->dtype, 1, 0, (hipStream_t)stream);
 }
 
 extern "C" int pxg_decay_backward(const pxg_decay* a, void* stream)
@@ -216,28 +194,32 @@ extern "C" int pxg_decay_backward(const pxg_decay* a, void* stream)
     if (bad_shape(a) || bad_operands(a)) return PXG_E_INVALID;
     const bool any = a->batch > 0 && a->steps > 0;
     if (any && (!a->grad_q || !a->grad_k || !a->grad_v || !a->grad_out.data)) return PXG_E_INVALID;
-    if (a->workspace_bytes < pxg_decay_workspace_bytes(a, 1) || (a->batch > 0 && !a->workspace)) return PXG_E_INVALID;
+    const int64_t bytes = pxg_decay_workspace_bytes(a, 1);
+    if (a->workspace_bytes < bytes || (bytes > 0 && !a->workspace)) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
-    const DecayShape s = shape_of(a);
+    const Cut c = cut_of(a);
+    DecayRuns s = runs_of(a, c);
+    float* const partial = (float*)a->workspace + 4 * carry_values(a, c);
     int rc = PXG_OK;
     if (a->batch > 0) {
-        DecayRun dq = {}, dk = {}, dv = {};
+        DecayRun &dq = s.run[0], &dk = s.run[1], &dv = s.run[2];
         dq.x = a->grad_out, dq.y = a->v, dq.z = a->k;
         dq.init = a->initial_state, dq.init_e = 1, dq.init_f = a->dv;
         dq.out = a->grad_q, dq.E = a->dv, dq.F = a->dk;
-        if (a->grad_log_decay) dq.dot = a->q, dq.grad_fin = a->grad_final_state, dq.partial = (float*)a->workspace;
+        if (a->grad_log_decay) dq.dot = a->q, dq.grad_fin = a->grad_final_state, dq.partial = partial;
         dk.x = a->v, dk.y = a->grad_out, dk.z = a->q, dk.reverse = 1;
         dk.init = a->grad_final_state, dk.init_e = 1, dk.init_f = a->dv;
         dk.out = a->grad_k, dk.E = a->dv, dk.F = a->dk;
         dv.x = a->k, dv.y = a->q, dv.z = a->grad_out, dv.reverse = 1;
         dv.init = a->grad_final_state, dv.fin = a->grad_initial_state, dv.init_e = a->dv, dv.init_f = 1;
         dv.out = a->grad_v, dv.E = a->dk, dv.F = a->dv;
-        rc = run(dq, s, a->dtype, st);
-        if (rc == PXG_OK) rc = run(dk, s, a->dtype, st);
-        if (rc == PXG_OK) rc = run(dv, s, a->dtype, st);
+        dq.carry = (float*)a->workspace;                                      // states and slopes
+        dk.carry = dq.carry + 2 * carry_values(a, c), dv.carry = dk.carry + carry_values(a, c);
+        for (DecayRun& r : s.run) finish_run(r, a->dtype);
+        rc = launch_runs(s, a->dtype, 3, a->grad_log_decay ? 1 : 0, st);
     }
     if (rc == PXG_OK && a->grad_log_decay) {
-        k_decay_sum<<<a->heads, 256, 0, st>>>((const float*)a->workspace, a->batch, a->heads, a->grad_log_decay);
+        k_decay_sum<<<a->heads, 256, 0, st>>>(partial, a->batch, a->heads, c.segments, a->grad_log_decay);
         if (hipGetLastError() != hipSuccess) rc = PXG_E_HIP;
     }
     return rc;

@@ -1,0 +1,8 @@
+// k_decay_f32.hip -- the chunked recurrence (k_decay_chunk.h) for one element type: a source of its own, so that the types compile
+// side by side.
+#include "k_decay_chunk.h"
+
+int decay_launch_f32(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream)
+{
+    return decay::launch<float>(a, first, n, slope, states_only, stream);
+}

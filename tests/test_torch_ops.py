@@ -546,7 +546,7 @@ def test_distillation_loss_strange_rows():
     assert torch.isnan(ops.distillation_loss(x.cuda(), teacher.to('cuda')))
     empty = ops.TopLogits(torch.empty(0, 3, device='cuda'), torch.empty(0, 3, dtype=torch.int32, device='cuda'))
     none = torch.empty(0, 9, device='cuda', requires_grad=True)
-    assert float(ops.distillation_loss(none, empty, reduction='sum')) == 0
+    assert float(ops.distillation_loss(none.detach(), empty, reduction='sum')) == 0
 
 
 # ---- together, streams, graphs ----------------------------------------------------------------------------------------------
