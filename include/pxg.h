@@ -731,7 +731,7 @@ typedef struct {
     int32_t grad_per_row;             /* backward: grad_loss is [rows] (of row_loss) instead of one value (of loss) */
     float* row_loss;                  /* [rows] */
     float* loss;                      /* one value, or NULL: not wanted */
-    float* stats;                     /* [rows][4]: what the backward pass needs of the forward pass */
+    float* stats;                     /* [rows][4 + k]: what the backward pass needs of the forward pass */
     const float* grad_loss;
     void* grad_logits;                /* [rows][classes] contiguous */
 } pxg_distill;

@@ -5,14 +5,49 @@
 // Student: z = log sum_v exp(x_v / temperature); q_i = exp(x_i / temperature - z) of a listed class, q_r the sum over the others.
 //   L = temperature^2 sum_i p_i (log p_i - log q_i),   dL/dx_v = temperature (q_v - p_v)            v listed
 //                                                      dL/dx_v = temperature q_v (1 - p_r / q_r)    v unlisted
-// The sum over the classes is taken in float32 against its own maximum; the k + 1 shares of a row are combined in float64, where
-// the difference of nearly equal unlisted shares (few listed classes, a high temperature) keeps its digits.
+// The sum over the classes is taken in float32 against its own running maximum, in one pass over the row; the k + 1 shares of a
+// row are combined in float64, where the difference of nearly equal unlisted shares (few listed classes, a high temperature)
+// keeps its digits.
+//
+// All of them are bound by reading the logits once (and writing the gradient once): a row belongs to one wave, to four or to
+// sixteen, by its length and the number of rows, and every lane reads 16 bytes at a time, four times before it computes.
 #include "pxg_ops.h"
 
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int AHEAD = 4;                      // 16-byte loads of a lane in flight
 
+// ---- a group of G threads (one wave, or the whole workgroup) that shares a row ------------------------------------------------
+template <int G> __device__ __forceinline__ void group_sync()
+{
+    if constexpr (G == 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
+    }
+}
+
+struct MaxOf { template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
+struct SumOf { template <typename V> __device__ V operator()(V a, V b) const { return a + b; } };
+
+// every thread gets the result; `lds` holds G / 64 values and may be used again at once
+template <int G, typename V, typename F> __device__ __forceinline__ V group_reduce(V v, V* lds, F f)
+{
+#pragma unroll
+    for (int m = 32; m; m >>= 1) v = f(v, __shfl_xor(v, m));
+    if constexpr (G > 64) {
+        __syncthreads();
+        if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
+        __syncthreads();
+        v = lds[0];
+#pragma unroll
+        for (int w = 1; w < G / 64; w++) v = f(v, lds[w]);
+    }
+    return v;
+}
+
+// ---- numbers --------------------------------------------------------------------------------------------------------------------
 // floats in the order of their values as unsigned integers: -0 as +0, NaN above everything
 __device__ __forceinline__ uint32_t order_of(float x)
 {
@@ -43,217 +78,544 @@ __device__ __forceinline__ Scale scale_of(float temperature)
 
 __device__ __forceinline__ float exp_from(float x, float base, Scale s)
 {
-    const float d = x - base;
-    return __builtin_amdgcn_exp2f(fmaf(d, s.hi, d * s.lo));
+    const float d = x - base;                   // may be -inf: not times a number that may be 0 or below
+    return __builtin_amdgcn_exp2f(fmaf(d, s.hi, __builtin_amdgcn_fmed3f(d, -1e30f, 1e30f) * s.lo));
 }
 
-template <typename V, typename F> __device__ __forceinline__ V block_reduce(V v, V* lds, F f)
+// 16 bytes of a row, which may begin anywhere; -inf behind its end
+template <typename T> struct Unit {
+    static constexpr int n = 16 / sizeof(T);
+    T v[n];
+};
+
+template <typename T> __device__ __forceinline__ Unit<T> load_unit(const T* x, int64_t unit, int64_t classes)
 {
-    __syncthreads();
-    lds[threadIdx.x] = v;
-    __syncthreads();
-    for (int w = THREADS / 2; w; w >>= 1) {
-        if ((int)threadIdx.x < w) lds[threadIdx.x] = f(lds[threadIdx.x], lds[threadIdx.x + w]);
-        __syncthreads();
+    constexpr int n = Unit<T>::n;
+    Unit<T> u;
+    if ((unit + 1) * n <= classes) {
+        __builtin_memcpy(&u, x + unit * n, sizeof u);
+    } else {
+#pragma unroll
+        for (int e = 0; e < n; e++) u.v[e] = unit * n + e < classes ? x[unit * n + e] : (T)-INFINITY;
     }
-    return lds[0];
+    return u;
 }
 
-struct MaxOf { template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
-struct SumOf { template <typename V> __device__ V operator()(V a, V b) const { return a + b; } };
-
-template <typename T>
-__global__ __launch_bounds__(THREADS) void k_top(int64_t classes, const T* logits, int64_t row_stride, int k, float temperature,
-                                                T* values, int32_t* indices, float* rest)
+// calls f(first class, floats) for the units of a row that are this thread's
+template <int G, typename T, typename F> __device__ __forceinline__ void each_unit(const T* x, int64_t classes, int t, F f)
 {
-    __shared__ unsigned long long red[THREADS];
-    __shared__ float redf[THREADS];
-    const int64_t row = blockIdx.x;
+    constexpr int n = Unit<T>::n;
+    const int64_t units = (classes + n - 1) / n;
+    for (int64_t i = t; i < units; i += G * AHEAD) {
+        Unit<T> u[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) u[a] = load_unit(x, i + a * G, classes);
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) {
+            float v[n];
+#pragma unroll
+            for (int e = 0; e < n; e++) v[e] = pxg_to_f32(u[a].v[e]);
+            if (i + a * G < units) f((i + a * G) * n, v);
+        }
+    }
+}
+
+// ---- the largest logits ---------------------------------------------------------------------------------------------------------
+// Each of the G threads knows the largest of its own elements; the k-th largest of these G is a bound that at least k elements
+// reach, and about -G log(1 - k / G) of evenly spread ones (k = 128, G = 256: 177).  A second pass (the row is still in a cache)
+// collects the elements at or above the bound and sums up the others; the candidates are ranked by counting.  Rows with more
+// candidates than CAND (plateaus of equal values) take their bound by bisection.
+constexpr int CAND = 1024;
+
+template <int G> struct alignas(16) TopShared {
+    unsigned long long cand[CAND];              // (order, ~class): no two are equal
+    uint32_t most[G];
+    float redf[G / 64];
+    int red[G / 64];
+    double redd[G / 64];
+    int count;
+    uint32_t bound;
+};
+
+template <int G, typename T>
+__global__ __launch_bounds__(G == 64 ? 256 : G)
+void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, int k, float temperature, T* values, int32_t* indices,
+           float* rest)
+{
+    constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n;
+    __shared__ TopShared<G> shared[GROUPS];
+    const int64_t row = (int64_t)blockIdx.x * GROUPS + (G == 64 ? threadIdx.x / 64 : 0);
+    if (row >= rows) return;                    // a whole wave, or nobody
+    TopShared<G>& s = shared[G == 64 ? threadIdx.x / 64 : 0];
+    const int t = threadIdx.x % G;
     const T* x = logits + row * row_stride;
-    // (order, classes - index) of the last one chosen: the next is the largest pair below it
-    unsigned long long last = ~0ull;
-    for (int i = 0; i < k; i++) {
-        unsigned long long best = 0;
-        for (int64_t v = threadIdx.x; v < classes; v += THREADS) {
-            const unsigned long long key = (unsigned long long)order_of(pxg_to_f32(x[v])) << 32 | (uint32_t)(classes - v);
-            if (key < last && key > best) best = key;
+    const Scale scale = scale_of(temperature);
+
+    uint32_t mine = 0;
+    {
+        float most = -INFINITY;
+        bool strange = false;
+        if (classes < (int64_t)G * n) {         // one element after the other: min(G, classes) threads have some, k at least
+            for (int64_t v = t; v < classes; v += G) {
+                const float f = pxg_to_f32(x[v]);
+                most = fmaxf(most, f), strange |= f != f;
+            }
+        } else {
+            each_unit<G>(x, classes, t, [&](int64_t, const float* v) {
+#pragma unroll
+                for (int e = 0; e < n; e++) most = fmaxf(most, v[e]), strange |= v[e] != v[e];
+            });
         }
-        last = block_reduce(best, red, MaxOf());
-        if (threadIdx.x == 0) {
-            const int64_t v = classes - (int64_t)(last & 0xffffffffu);
-            values[row * k + i] = x[v];
-            indices[row * k + i] = (int32_t)v;
+        mine = strange ? 0xffffffffu : order_of(most);
+    }
+    s.most[t] = mine;
+    if (t == 0) s.count = 0;
+    group_sync<G>();
+    {
+        int ahead = 0;
+        for (int i = 0; i < G; i += 4) {
+            const uint4 o = *(const uint4*)(s.most + i);
+            ahead += (o.x > mine || (o.x == mine && i < t)) + (o.y > mine || (o.y == mine && i + 1 < t)) +
+                     (o.z > mine || (o.z == mine && i + 2 < t)) + (o.w > mine || (o.w == mine && i + 3 < t));
         }
+        if (ahead == k - 1) s.bound = mine;
     }
-    uint32_t most = 0;
-    for (int64_t v = threadIdx.x; v < classes; v += THREADS) {
-        const unsigned long long key = (unsigned long long)order_of(pxg_to_f32(x[v])) << 32 | (uint32_t)(classes - v);
-        if (key < last && (uint32_t)(key >> 32) > most) most = (uint32_t)(key >> 32);
+    group_sync<G>();
+    uint32_t bound_key = s.bound;
+    float bound = value_of(bound_key), most = -INFINITY, sum = 0.f, base = __builtin_isfinite(bound) ? bound : 0.f;
+    // everything below the bound: its largest element, and its sum against the bound
+    each_unit<G>(x, classes, t, [&](int64_t first, const float* v) {
+#pragma unroll
+        for (int e = 0; e < n; e++) {
+            if (v[e] < bound) {
+                most = fmaxf(most, v[e]);
+                sum += exp_from(v[e], base, scale);
+            } else if (first + e < classes) {
+                const int at = atomicAdd(&s.count, 1);
+                if (at < CAND) s.cand[at] = (unsigned long long)order_of(v[e]) << 32 | (uint32_t)~(uint32_t)(first + e);
+            }
+        }
+    });
+    group_sync<G>();
+    int found = s.count;
+    bool no_number = false;                     // among the rest (bisection only: otherwise it is a candidate)
+    uint32_t before = 0xffffffffu;              // of the elements AT the bound, the classes below this one belong to the chosen
+    if (found > CAND) {
+        // the largest key that k elements reach, bit by bit; then the smallest class below which enough of the ties lie
+        const auto count = [&](auto is) {
+            int c = 0;
+            each_unit<G>(x, classes, t, [&](int64_t first, const float* v) {
+#pragma unroll
+                for (int e = 0; e < n; e++)
+                    if (first + e < classes && is(order_of(v[e]), (uint32_t)(first + e))) c++;
+            });
+            return group_reduce<G>(c, s.red, SumOf());
+        };
+        uint32_t key = 0;
+        for (int bit = 31; bit >= 0; bit--) {
+            const uint32_t next = key | 1u << bit;
+            if (count([&](uint32_t o, uint32_t) { return o >= next; }) >= k) key = next;
+        }
+        const int need = k - count([&](uint32_t o, uint32_t) { return o > key; });
+        uint32_t low = 0, high = (uint32_t)classes;                 // count(low) < need <= count(high)
+        while (high - low > 1) {
+            const uint32_t mid = low + (high - low) / 2;
+            if (count([&](uint32_t o, uint32_t c) { return o == key && c < mid; }) >= need) high = mid;
+            else low = mid;
+        }
+        bound_key = key, before = high, found = k;
+        if (t == 0) s.count = 0;
+        group_sync<G>();
+        most = -INFINITY;
+        bool strange = false;
+        each_unit<G>(x, classes, t, [&](int64_t first, const float* v) {
+#pragma unroll
+            for (int e = 0; e < n; e++) {
+                const uint32_t o = order_of(v[e]);
+                if (first + e >= classes) continue;
+                if (o > bound_key || (o == bound_key && (uint32_t)(first + e) < before))
+                    s.cand[atomicAdd(&s.count, 1)] = (unsigned long long)o << 32 | (uint32_t)~(uint32_t)(first + e);
+                else
+                    most = fmaxf(most, v[e]), strange |= v[e] != v[e];
+            }
+        });
+        no_number = group_reduce<G>((int)strange, s.red, MaxOf());
+        group_sync<G>();
     }
-    most = (uint32_t)block_reduce((unsigned long long)most, red, MaxOf());
-    const float base = value_of(most);
-    const Scale s = scale_of(temperature);
-    float sum = 0.f;
-    for (int64_t v = threadIdx.x; v < classes; v += THREADS) {
-        const float f = pxg_to_f32(x[v]);
-        const unsigned long long key = (unsigned long long)order_of(f) << 32 | (uint32_t)(classes - v);
-        if (key < last) sum += exp_from(f, base, s);
+    const bool by_bisection = before != 0xffffffffu;
+    most = group_reduce<G>(most, s.redf, MaxOf());
+    // the bound may lie far above what is below it (or be no number): sum up against that instead
+    if (by_bisection || !__builtin_isfinite(bound) || (bound - most) * scale.hi > 64.f) {
+        base = most, sum = 0.f;
+        if (__builtin_isfinite(base))
+            each_unit<G>(x, classes, t, [&](int64_t first, const float* v) {
+#pragma unroll
+                for (int e = 0; e < n; e++) {
+                    const uint32_t o = order_of(v[e]);
+                    if (o < bound_key || (by_bisection && o == bound_key && (uint32_t)(first + e) >= before))
+                        sum += exp_from(v[e], base, scale);
+                }
+            });
     }
-    sum = block_reduce(sum, redf, SumOf());
-    if (threadIdx.x == 0)
-        rest[row] = most == 0 || base == -INFINITY ? -INFINITY : base == INFINITY ? INFINITY
-                                                   : (float)((double)base / (double)temperature + log((double)sum));
+    const double below = group_reduce<G>((double)sum, s.redd, SumOf());
+    // rank the candidates; the first k are the answer, the rest join the sum against the largest of them
+    double extra = 0.0;
+    const bool left = found > k;
+    if (left) {
+        if (t == 0) s.bound = 0;
+        group_sync<G>();
+    }
+    int rank[(CAND + G - 1) / G];
+#pragma unroll
+    for (int a = 0; a < (CAND + G - 1) / G; a++) {
+        const int i = t + a * G;
+        int ahead = 0;
+        if (i < found) {
+            const unsigned long long key = s.cand[i];
+            for (int j = 0; j < found; j++) ahead += s.cand[j] > key;
+            if (ahead < k) {
+                const int64_t at = (int64_t)(uint32_t)~(uint32_t)key;
+                values[row * k + ahead] = x[at];
+                indices[row * k + ahead] = (int32_t)at;
+            } else if (ahead == k) {
+                s.bound = (uint32_t)(key >> 32);
+            }
+        }
+        rank[a] = ahead;
+    }
+    float top = base;
+    if (left) {
+        group_sync<G>();
+        top = value_of(s.bound);
+        if (__builtin_isfinite(top)) {
+#pragma unroll
+            for (int a = 0; a < (CAND + G - 1) / G; a++)
+                if (t + a * G < found && rank[a] >= k)
+                    extra += exp(((double)value_of((uint32_t)(s.cand[t + a * G] >> 32)) - (double)top) / (double)temperature);
+        }
+        extra = group_reduce<G>(extra, s.redd, SumOf());
+    }
+    if (t == 0) {
+        double r;
+        if (left && !__builtin_isfinite(top)) r = top;                     // -inf: so is all the rest
+        else if (left) r = (double)top / temperature + log(extra + (below > 0.0 ? below * exp(((double)base - top) / temperature) : 0.0));
+        else if (no_number) r = NAN;
+        else if (!(most > -INFINITY)) r = -INFINITY;
+        else if (!__builtin_isfinite(most)) r = INFINITY;
+        else r = (double)base / temperature + log(below);
+        rest[row] = (float)r;
+    }
 }
 
+// ---- the loss -------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ double number_at(const void* p, int64_t i, int dtype)
 {
     return dtype == PXG_DT_F32 ? (double)((const float*)p)[i]
          : dtype == PXG_DT_BF16 ? (double)(float)((const pxg_bf16*)p)[i] : (double)(float)((const pxg_f16*)p)[i];
 }
 
-// A row's listed classes in shared memory: index (-1: empty place or an earlier place holds the class; then `share` is 0 and the
-// first place has the sum) and the teacher's share.
-struct Listed {
-    int64_t index[PXG_TOP_MAX_K];
-    double share[PXG_TOP_MAX_K], raw[PXG_TOP_MAX_K], rest_share;
-    int bad, none;
+// Which classes of a row are listed: one bit for each 16-byte unit of the row (more units share a bit in rows of more than
+// 32 768 of them), and a table of the units that hold listed classes.
+template <int G> struct Marks {
+    static constexpr int words = G == 64 ? 64 : 1024, slots = 256;
+    uint32_t filter[words];
+    int32_t unit[slots];
+    uint32_t mask[slots];
+
+    __device__ void clear(int t)
+    {
+        for (int i = t; i < words; i += G) filter[i] = 0;
+        for (int i = t; i < slots; i += G) unit[i] = -1, mask[i] = 0;
+    }
+    static __device__ int slot_of(int32_t u) { return (int)((uint32_t)u * 2654435761u >> 24); }
+    __device__ void add(int64_t index, int n)                     // at most PXG_TOP_MAX_K of them: there is always a free slot
+    {
+        const int32_t u = (int32_t)(index / n);
+        atomicOr(&filter[(u >> 5) & (words - 1)], 1u << (u & 31));
+        for (int s = slot_of(u);; s = (s + 1) & (slots - 1)) {
+            const int32_t was = atomicCAS(&unit[s], -1, u);
+            if (was == -1 || was == u) {
+                atomicOr(&mask[s], 1u << (index % n));
+                return;
+            }
+        }
+    }
+    __device__ __forceinline__ uint32_t of(int32_t u) const
+    {
+        if (!(filter[(u >> 5) & (words - 1)] >> (u & 31) & 1)) return 0;
+        for (int s = slot_of(u);; s = (s + 1) & (slots - 1)) {
+            const int32_t is = unit[s];
+            if (is == u) return mask[s];
+            if (is < 0) return 0;
+        }
+    }
 };
 
-__device__ void read_teacher(const pxg_distill& a, int64_t row, Listed& l, double* red)
+template <int G> struct LossShared {
+    Marks<G> marks;
+    int32_t index[PXG_TOP_MAX_K];               // -1: an empty place, or an earlier one holds the class
+    double share[PXG_TOP_MAX_K];
+    double redd[G / 64];
+    float redf[G / 64];
+    int red[G / 64];
+};
+
+// `stats` of a row: the unlisted classes' maximum, the factor of their exponentials in the gradient, whether the row counts (0: no,
+// 1: yes, NaN: it names what is no class), unused, then q - p of each place (+inf: no class's first place)
+constexpr int STATS = 4;
+
+template <int G, typename T>
+__global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_forward(const pxg_distill a)
 {
-    const int i = threadIdx.x;
-    double t = -INFINITY;
-    int64_t index = -1;
-    if (i == 0) l.bad = 0;
-    __syncthreads();
-    if (i < a.k) {
-        index = a.indices_are_64 ? ((const int64_t*)a.indices)[row * a.k + i] : ((const int32_t*)a.indices)[row * a.k + i];
-        if (index < -1 || index >= a.classes) l.bad = 1, index = -1;
-        else if (index >= 0) t = number_at(a.values, row * a.k + i, a.value_dtype) / (double)a.temperature;
-        l.index[i] = index;
+    constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n, PLACES = (PXG_TOP_MAX_K + G - 1) / G;
+    __shared__ LossShared<G> shared[GROUPS];
+    const int64_t row = (int64_t)blockIdx.x * GROUPS + (G == 64 ? threadIdx.x / 64 : 0);
+    if (row >= a.rows) return;
+    LossShared<G>& s = shared[G == 64 ? threadIdx.x / 64 : 0];
+    const int t = threadIdx.x % G, k = a.k;
+    float* stats = a.stats + row * (STATS + k);
+    const double w = a.weight ? (double)a.weight[row] : 1.0, tau = a.temperature;
+    const T* x = (const T*)a.logits + row * a.row_stride;
+
+    // the teacher's shares
+    s.marks.clear(t);
+    int bad = 0;
+    double value[PLACES], most = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < PLACES; p++) {
+        const int i = t + p * G;
+        value[p] = -INFINITY;
+        if (i < k) {
+            const int64_t at = row * k + i;
+            int64_t index = a.indices_are_64 ? ((const int64_t*)a.indices)[at] : ((const int32_t*)a.indices)[at];
+            if (index < -1 || index >= a.classes) bad = 1, index = -1;
+            if (index >= 0) value[p] = number_at(a.values, at, a.value_dtype) / tau;
+            s.index[i] = (int32_t)index;
+            most = value[p] > most ? value[p] : most;
+        }
     }
     const double rest = a.rest ? (double)a.rest[row] : -INFINITY;
-    double base = block_reduce(t, red, MaxOf());
-    if (rest > base) base = rest;
-    const double e = t == -INFINITY ? 0.0 : exp(t - base), er = rest == -INFINITY ? 0.0 : exp(rest - base);
-    const double total = block_reduce(e, red, SumOf()) + er;
-    if (i < a.k) l.raw[i] = total > 0.0 || total != total ? e / total : 0.0;
-    if (i == 0) l.rest_share = total > 0.0 || total != total ? er / total : 0.0, l.none = total == 0.0;
-    __syncthreads();
-    // every thread takes every barrier: the first place of a class takes the shares of all of them
+    bad = group_reduce<G>(bad, s.red, MaxOf());
+    double top = group_reduce<G>(most, s.redd, MaxOf());
+    top = rest > top ? rest : top;
     double sum = 0.0;
-    bool first = index >= 0;
-    for (int j = 0; i < a.k && index >= 0 && j < a.k; j++)
-        if (l.index[j] == index) {
-            if (j < i) first = false;
-            sum += l.raw[j];
-        }
-    __syncthreads();
-    if (i < a.k) {
-        l.share[i] = first ? sum : 0.0;
-        if (!first) l.index[i] = -1;
+#pragma unroll
+    for (int p = 0; p < PLACES; p++) {
+        value[p] = value[p] == -INFINITY ? 0.0 : exp(value[p] - top);
+        sum += value[p];
     }
-    __syncthreads();
-}
-
-template <typename T>
-__global__ __launch_bounds__(THREADS) void k_distill_forward(pxg_distill a)
-{
-    __shared__ Listed l;
-    __shared__ double red[THREADS];
-    __shared__ float redf[THREADS];
-    const int64_t row = blockIdx.x;
-    const double w = a.weight ? (double)a.weight[row] : 1.0;
-    float* stats = a.stats + row * 4;
-    if (w != 0.0) read_teacher(a, row, l, red);
-    if (w == 0.0 || (l.none && !l.bad)) {
-        if (threadIdx.x == 0) {
-            a.row_loss[row] = 0.f;
-            stats[0] = stats[1] = stats[2] = stats[3] = 0.f;
-        }
+    const double rest_exp = rest == -INFINITY ? 0.0 : exp(rest - top);
+    const double total_p = group_reduce<G>(sum, s.redd, SumOf()) + rest_exp;
+    if (w == 0.0 || (total_p == 0.0 && !bad)) {                   // the whole group
+        if (t == 0) stats[2] = 0.f, a.row_loss[row] = 0.f;
         return;
     }
-    const T* x = (const T*)a.logits + row * a.row_stride;
-    const Scale s = scale_of(a.temperature);
-    float most = -INFINITY, sum = 0.f;
-    for (int64_t v = threadIdx.x; v < a.classes; v += THREADS) {
-        bool listed = false;
-        for (int i = 0; i < a.k; i++) listed |= l.index[i] == v;
-        const float f = pxg_to_f32(x[v]);
-        if (!listed && (f > most || f != f)) most = f;
+    const double p_rest = rest_exp / total_p;
+#pragma unroll
+    for (int p = 0; p < PLACES; p++)
+        if (t + p * G < k) s.share[t + p * G] = value[p] / total_p;
+    group_sync<G>();
+    // a class that is listed more than once: its first place takes all its shares
+    double share[PLACES];
+    bool first[PLACES];
+#pragma unroll
+    for (int p = 0; p < PLACES; p++) {
+        const int i = t + p * G;
+        const int32_t index = i < k ? s.index[i] : -1;
+        share[p] = 0.0, first[p] = index >= 0;
+        if (index >= 0) {
+            for (int j = 0; j < k; j++)
+                if (s.index[j] == index) {
+                    if (j < i) first[p] = false;
+                    share[p] += s.share[j];
+                }
+            s.marks.add(index, n);
+        }
     }
-    const float base_u = block_reduce(most, redf, MaxOf());
-    for (int64_t v = threadIdx.x; v < a.classes; v += THREADS) {
-        bool listed = false;
-        for (int i = 0; i < a.k; i++) listed |= l.index[i] == v;
-        const float f = pxg_to_f32(x[v]);
-        if (!listed && f != -INFINITY) sum += exp_from(f, base_u, s);
+    group_sync<G>();
+
+    // the student's unlisted classes: running maximum and sum
+    const Scale scale = scale_of(a.temperature);
+    float base_u = -3.402823466e38f, sum_u = 0.f;
+    {
+        const int64_t units = (a.classes + n - 1) / n;
+        for (int64_t i = t; i < units; i += G * AHEAD) {
+            Unit<T> u[AHEAD];
+            float v[AHEAD][n], next = base_u;
+#pragma unroll
+            for (int b = 0; b < AHEAD; b++) u[b] = load_unit(x, i + b * G, a.classes);
+#pragma unroll
+            for (int b = 0; b < AHEAD; b++) {
+                const uint32_t mask = i + b * G < units ? s.marks.of((int32_t)(i + b * G)) : 0;
+#pragma unroll
+                for (int e = 0; e < n; e++) v[b][e] = pxg_to_f32(u[b].v[e]);
+                if (mask)
+#pragma unroll
+                    for (int e = 0; e < n; e++)
+                        if (mask >> e & 1) v[b][e] = -INFINITY;
+#pragma unroll
+                for (int e = 0; e < n; e++) next = fmaxf(next, v[b][e]);
+            }
+            if (next > base_u) sum_u *= exp_from(base_u, next, scale), base_u = next;
+#pragma unroll
+            for (int b = 0; b < AHEAD; b++)
+#pragma unroll
+                for (int e = 0; e < n; e++) sum_u += exp_from(v[b][e], base_u, scale);
+        }
     }
-    const double sum_u = block_reduce(sum, redf, SumOf());
+    const float all_u = group_reduce<G>(base_u, s.redf, MaxOf());
+    // (a thread without any keeps its sum of 0 whatever its exponent says)
+    const double unlisted = group_reduce<G>(sum_u == 0.f ? 0.0 : (double)sum_u * (double)exp_from(base_u, all_u, scale), s.redd, SumOf());
+
     // the k + 1 shares
-    const int i = threadIdx.x;
-    const bool mine = i < a.k && l.index[i] >= 0;
-    const double xi = mine ? (double)pxg_to_f32(x[l.index[i]]) : -INFINITY;
-    double base = block_reduce(xi, red, MaxOf());
-    if ((double)base_u > base) base = base_u;
-    const double tau = a.temperature, u = sum_u == 0.0 ? 0.0 : sum_u * exp(((double)base_u - base) / tau);
-    const double total = block_reduce(mine ? exp((xi - base) / tau) : 0.0, red, SumOf()) + u;
-    const double log_total = log(total);
+    double xi[PLACES], base = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < PLACES; p++) {
+        xi[p] = first[p] ? (double)pxg_to_f32(x[s.index[t + p * G]]) : -INFINITY;
+        base = xi[p] > base ? xi[p] : base;
+    }
+    base = group_reduce<G>(base, s.redd, MaxOf());
+    if (unlisted != 0.0 && !((double)all_u <= base)) base = all_u;
+    double listed = 0.0;
+#pragma unroll
+    for (int p = 0; p < PLACES; p++) {
+        xi[p] = (xi[p] - base) / tau;
+        listed += first[p] ? exp(xi[p]) : 0.0;
+    }
+    const double far_u = ((double)all_u - base) / tau;
+    const double u = unlisted == 0.0 ? 0.0 : unlisted * exp(far_u);
+    const double total = group_reduce<G>(listed, s.redd, SumOf()) + u, log_total = log(total);
     double term = 0.0;
-    if (mine && l.share[i] != 0.0) term = l.share[i] * (log(l.share[i]) - ((xi - base) / tau - log_total));
-    double loss = block_reduce(term, red, SumOf());
-    if (i == 0) {
-        const double pr = l.rest_share;
-        if (pr != 0.0) loss += pr * (log(pr) - (log(sum_u) + ((double)base_u - base) / tau - log_total));
-        if (l.bad) loss = NAN;
+#pragma unroll
+    for (int p = 0; p < PLACES; p++) {
+        const int i = t + p * G;
+        if (first[p] && share[p] != 0.0) term += share[p] * (log(share[p]) - (xi[p] - log_total));
+        if (i < k) stats[STATS + i] = first[p] ? (float)(exp(xi[p]) / total - share[p]) : INFINITY;
+    }
+    double loss = group_reduce<G>(term, s.redd, SumOf());
+    if (t == 0) {
+        if (p_rest != 0.0) loss += p_rest * (log(p_rest) - (log(unlisted) + far_u - log_total));
+        if (bad) loss = NAN;
         a.row_loss[row] = (float)(w * tau * tau * loss);
-        stats[0] = base_u;
-        stats[1] = sum_u == 0.0 ? 0.f : (float)((u / total - pr) / sum_u);
-        stats[2] = (float)base;
-        stats[3] = l.bad ? NAN : (float)total;
+        stats[0] = all_u;
+        stats[1] = unlisted == 0.0 ? 0.f : (float)((u / total - p_rest) / unlisted);
+        stats[2] = bad ? NAN : 1.f;
+        stats[3] = 0.f;
     }
 }
 
-__global__ __launch_bounds__(THREADS) void k_distill_sum(const float* row_loss, int64_t rows, int mean, float* loss)
+__global__ __launch_bounds__(256) void k_distill_sum(const float* row_loss, int64_t rows, int mean, float* loss)
 {
-    __shared__ double red[THREADS];
+    __shared__ double red[4];
     double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < rows; i += THREADS) sum += (double)row_loss[i];
-    sum = block_reduce(sum, red, SumOf());
+    for (int64_t i = threadIdx.x; i < rows; i += 256) sum += (double)row_loss[i];
+    sum = group_reduce<256>(sum, red, SumOf());
     if (threadIdx.x == 0) *loss = (float)(mean ? sum / (double)rows : sum);
 }
 
-template <typename T>
-__global__ __launch_bounds__(THREADS) void k_distill_backward(pxg_distill a)
+template <int G, typename T>
+__global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_backward(const pxg_distill a)
 {
-    __shared__ Listed l;
-    __shared__ double red[THREADS];
-    const int64_t row = blockIdx.x;
-    const double w = a.weight ? (double)a.weight[row] : 1.0;
-    const float* stats = a.stats + row * 4;
-    const float base_u = stats[0], c = stats[1], base = stats[2], total = stats[3];
-    T* g = (T*)a.grad_logits + row * a.classes;
-    if (w == 0.0 || total == 0.f) {
-        for (int64_t v = threadIdx.x; v < a.classes; v += THREADS) g[v] = pxg_from_f32<T>(0.f);
-        return;
-    }
-    read_teacher(a, row, l, red);
-    const double tau = a.temperature;
-    const double factor = w * tau * (double)a.grad_loss[a.grad_per_row ? row : 0] / (a.mean && !a.grad_per_row ? (double)a.rows : 1.0);
+    constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n;
+    __shared__ Marks<G> shared[GROUPS];
+    const int64_t row = (int64_t)blockIdx.x * GROUPS + (G == 64 ? threadIdx.x / 64 : 0);
+    if (row >= a.rows) return;
+    Marks<G>& marks = shared[G == 64 ? threadIdx.x / 64 : 0];
+    const int t = threadIdx.x % G, k = a.k;
+    const float* stats = a.stats + row * (STATS + k);
+    const float counts = stats[2], base_u = stats[0], c = stats[1];
     const T* x = (const T*)a.logits + row * a.row_stride;
-    const Scale s = scale_of(a.temperature);
-    const float fc = l.bad ? NAN : (float)(factor * c);
-    for (int64_t v = threadIdx.x; v < a.classes; v += THREADS) {
-        int at = -1;
-        for (int i = 0; i < a.k; i++)
-            if (l.index[i] == v) at = i;
-        const float f = pxg_to_f32(x[v]);
-        float r;
-        if (at < 0)
-            r = f == -INFINITY ? 0.f * fc : exp_from(f, base_u, s) * fc;
-        else
-            r = (float)(factor * (exp(((double)f - (double)base) / tau) / (double)total - l.share[at]));
-        g[v] = pxg_from_f32<T>(r);
+    T* g = (T*)a.grad_logits + row * a.classes;
+    const double w = a.weight ? (double)a.weight[row] : 1.0;
+    const double factor = counts == 0.f ? 0.0
+        : counts * w * (double)a.temperature * (double)a.grad_loss[a.grad_per_row ? row : 0] / (a.mean && !a.grad_per_row ? (double)a.rows : 1.0);
+    const float fc = counts == 0.f ? 0.f : (float)(factor * c);
+    const Scale scale = scale_of(a.temperature);
+    if (counts != 0.f) {
+        marks.clear(t);
+        group_sync<G>();
+        for (int i = t; i < k; i += G) {
+            const float d = stats[STATS + i];
+            if (d == INFINITY) continue;
+            const int64_t at = row * k + i, index = a.indices_are_64 ? ((const int64_t*)a.indices)[at] : ((const int32_t*)a.indices)[at];
+            marks.add(index, n);
+            g[index] = pxg_from_f32<T>((float)(factor * (double)d));
+        }
+        group_sync<G>();
+    }
+    const int64_t units = (a.classes + n - 1) / n;
+    for (int64_t i = t; i < units; i += G * AHEAD) {
+        Unit<T> u[AHEAD];
+        if (counts != 0.f) {
+#pragma unroll
+            for (int b = 0; b < AHEAD; b++) u[b] = load_unit(x, i + b * G, a.classes);
+        }
+#pragma unroll
+        for (int b = 0; b < AHEAD; b++) {
+            const int64_t unit = i + b * G;
+            if (unit >= units) continue;
+            uint32_t mask = 0;
+            if (counts != 0.f) {
+                mask = marks.of((int32_t)unit);
+#pragma unroll
+                for (int e = 0; e < n; e++) u[b].v[e] = pxg_from_f32<T>(exp_from(pxg_to_f32(u[b].v[e]), base_u, scale) * fc);
+            } else {
+#pragma unroll
+                for (int e = 0; e < n; e++) u[b].v[e] = pxg_from_f32<T>(0.f);
+            }
+            if (mask == 0 && (unit + 1) * n <= a.classes) {
+                __builtin_memcpy(g + unit * n, &u[b], sizeof u[b]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < n; e++)
+                    if (!(mask >> e & 1) && unit * n + e < a.classes) g[unit * n + e] = u[b].v[e];
+            }
+        }
+    }
+}
+
+// The threads that share a row: a wave for short ones, a workgroup of four waves, sixteen where there are too few rows to fill
+// the card with less.
+int threads_of(int64_t rows, int64_t classes)
+{
+    return classes <= 1024 ? 64 : rows < 512 && classes > 16384 ? 1024 : 256;
+}
+
+unsigned blocks_of(int64_t rows, int threads) { return (unsigned)(threads == 64 ? (rows + 3) / 4 : rows); }
+
+template <typename T>
+void launch_top(int64_t rows, int64_t classes, const void* logits, int64_t row_stride, int k, float temperature, void* values,
+                int32_t* indices, float* rest, hipStream_t st)
+{
+    int g = threads_of(rows, classes);
+    if (k > 32 && g == 64) g = 256;                               // twice as many threads as are to be chosen
+    const unsigned blocks = blocks_of(rows, g);
+    switch (g) {
+    case 64: k_top<64, T><<<blocks, 256, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest); break;
+    case 256: k_top<256, T><<<blocks, 256, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest); break;
+    default: k_top<1024, T><<<blocks, 1024, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest);
+    }
+}
+
+template <typename T> void launch_forward(const pxg_distill& a, hipStream_t st)
+{
+    const int g = threads_of(a.rows, a.classes);
+    const unsigned blocks = blocks_of(a.rows, g);
+    switch (g) {
+    case 64: k_distill_forward<64, T><<<blocks, 256, 0, st>>>(a); break;
+    case 256: k_distill_forward<256, T><<<blocks, 256, 0, st>>>(a); break;
+    default: k_distill_forward<1024, T><<<blocks, 1024, 0, st>>>(a);
+    }
+}
+
+template <typename T> void launch_backward(const pxg_distill& a, hipStream_t st)
+{
+    const int g = threads_of(a.rows, a.classes);
+    const unsigned blocks = blocks_of(a.rows, g);
+    switch (g) {
+    case 64: k_distill_backward<64, T><<<blocks, 256, 0, st>>>(a); break;
+    case 256: k_distill_backward<256, T><<<blocks, 256, 0, st>>>(a); break;
+    default: k_distill_backward<1024, T><<<blocks, 1024, 0, st>>>(a);
     }
 }
 
@@ -276,18 +638,10 @@ extern "C" int pxg_top_logits(int32_t dtype, int64_t rows, int64_t classes, cons
     if (rows == 0) return PXG_OK;
     if (!logits || !values || !indices || !rest) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
-    const int n = (int)rows;
     switch (dtype) {
-    case PXG_DT_F32:
-        k_top<float><<<n, THREADS, 0, st>>>(classes, (const float*)logits, row_stride, k, temperature, (float*)values, indices, rest);
-        break;
-    case PXG_DT_BF16:
-        k_top<pxg_bf16><<<n, THREADS, 0, st>>>(classes, (const pxg_bf16*)logits, row_stride, k, temperature, (pxg_bf16*)values,
-                                               indices, rest);
-        break;
-    default:
-        k_top<pxg_f16><<<n, THREADS, 0, st>>>(classes, (const pxg_f16*)logits, row_stride, k, temperature, (pxg_f16*)values,
-                                              indices, rest);
+    case PXG_DT_F32: launch_top<float>(rows, classes, logits, row_stride, k, temperature, values, indices, rest, st); break;
+    case PXG_DT_BF16: launch_top<pxg_bf16>(rows, classes, logits, row_stride, k, temperature, values, indices, rest, st); break;
+    default: launch_top<pxg_f16>(rows, classes, logits, row_stride, k, temperature, values, indices, rest, st);
     }
     return hipGetLastError() == hipSuccess ? PXG_OK : PXG_E_HIP;
 }
@@ -296,17 +650,16 @@ extern "C" int pxg_distill_forward(const pxg_distill* a, void* stream)
 {
     if (bad_call(a) || (a->rows > 0 && !a->row_loss)) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
-    const int n = (int)a->rows;
-    if (n) {
+    if (a->rows) {
         switch (a->dtype) {
-        case PXG_DT_F32: k_distill_forward<float><<<n, THREADS, 0, st>>>(*a); break;
-        case PXG_DT_BF16: k_distill_forward<pxg_bf16><<<n, THREADS, 0, st>>>(*a); break;
-        default: k_distill_forward<pxg_f16><<<n, THREADS, 0, st>>>(*a);
+        case PXG_DT_F32: launch_forward<float>(*a, st); break;
+        case PXG_DT_BF16: launch_forward<pxg_bf16>(*a, st); break;
+        default: launch_forward<pxg_f16>(*a, st);
         }
         if (hipGetLastError() != hipSuccess) return PXG_E_HIP;
     }
     if (a->loss) {
-        k_distill_sum<<<1, THREADS, 0, st>>>(a->row_loss, a->rows, a->mean, a->loss);
+        k_distill_sum<<<1, 256, 0, st>>>(a->row_loss, a->rows, a->mean, a->loss);
         if (hipGetLastError() != hipSuccess) return PXG_E_HIP;
     }
     return PXG_OK;
@@ -318,11 +671,10 @@ extern "C" int pxg_distill_backward(const pxg_distill* a, void* stream)
     if (a->rows == 0) return PXG_OK;
     if (!a->grad_loss || !a->grad_logits) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
-    const int n = (int)a->rows;
     switch (a->dtype) {
-    case PXG_DT_F32: k_distill_backward<float><<<n, THREADS, 0, st>>>(*a); break;
-    case PXG_DT_BF16: k_distill_backward<pxg_bf16><<<n, THREADS, 0, st>>>(*a); break;
-    default: k_distill_backward<pxg_f16><<<n, THREADS, 0, st>>>(*a);
+    case PXG_DT_F32: launch_backward<float>(*a, st); break;
+    case PXG_DT_BF16: launch_backward<pxg_bf16>(*a, st); break;
+    default: launch_backward<pxg_f16>(*a, st);
     }
     return hipGetLastError() == hipSuccess ? PXG_OK : PXG_E_HIP;
 }

@@ -392,9 +392,10 @@ def _distill_forward(code, logits, teacher, weight, reduction):
     s, keep = _distill_struct(code, logits, teacher, weight, reduction)
     device, rows = logits.device, logits.shape[0]
     none = reduction == 'none'
-    held = torch.empty(((4 if none else 5) * rows,), dtype=torch.float32, device=device)           # stats, row_loss
+    stats = rows * (4 + s.k)
+    held = torch.empty((stats + (0 if none else rows),), dtype=torch.float32, device=device)       # stats, row_loss
     loss = torch.empty((rows,) if none else (), dtype=torch.float32, device=device)
-    s.stats, s.row_loss = held.data_ptr(), loss.data_ptr() if none else held.data_ptr() + 16 * rows
+    s.stats, s.row_loss = held.data_ptr(), loss.data_ptr() if none else held.data_ptr() + 4 * stats
     if not none:
         s.loss = loss.data_ptr()
     _call(_lib().pxg_distill_forward, s, device)
