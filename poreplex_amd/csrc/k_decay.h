@@ -11,7 +11,7 @@ struct DecayRun {
     void* out;                 // [batch][steps][heads][F]
     int E, F;
     int reverse;               // steps taken from the last to the first; then init joins the first step without decay
-    int wide;                  // bits 0..3: rows of x, y, z, dot can be read 16 bytes at a time, bit 4: rows of out written 4 values at a time
+    int wide;                  // every row can be read 16 bytes and written four values at a time
     float* carry;              // states between segments, [batch * heads][segments - 1][E][F] (and the slopes behind them)
     // gradient of log_decay (the run of dq): q's rows, the gradient of the final state, one partial sum per (batch * heads, segment)
     pxg_sequence dot;

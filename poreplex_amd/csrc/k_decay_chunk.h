@@ -71,17 +71,29 @@ __device__ __forceinline__ bf16x4 read_transposed(const __bf16* p)
 // eight elements of a row on their way into shared memory
 template <typename T> struct Piece { T v[8]; };
 
-template <typename T> __device__ __forceinline__ Piece<T> load_piece(const T* row, int col, int width, bool wide, bool live)
+template <typename T> __device__ __forceinline__ Piece<T> load_wide(const T* at)
+{
+    Piece<T> p;
+    __builtin_memcpy(&p, __builtin_assume_aligned(at, 16), sizeof p);
+    return p;
+}
+
+template <typename T> __device__ __forceinline__ Piece<T> load_narrow(const T* row, int col, int width)
 {
     Piece<T> p = {};
-    if (wide) {
-        if (live && col < width) __builtin_memcpy(&p, __builtin_assume_aligned(row + col, 16), sizeof p);
-    } else if (live) {
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (col + e < width) p.v[e] = row[col + e];
-    }
+    for (int e = 0; e < 8; e++)
+        if (col + e < width) p.v[e] = row[col + e];
     return p;
+}
+
+template <typename T> __device__ __forceinline__ void clear_unless(bool keep, Piece<T>& p)
+{
+    uint4 w[sizeof p / 16];
+    __builtin_memcpy(w, &p, sizeof p);
+#pragma unroll
+    for (auto& v : w) v.x = keep ? v.x : 0, v.y = keep ? v.y : 0, v.z = keep ? v.z : 0, v.w = keep ? v.w : 0;
+    __builtin_memcpy(&p, w, sizeof p);
 }
 
 template <typename T, int PLANE> __device__ __forceinline__ void store_piece(const Piece<T>& p, __bf16* at)
@@ -113,7 +125,7 @@ __device__ __forceinline__ int xcd_order(int id, int n)
     return x * each + (x < more ? x : more) + id / 8;
 }
 
-template <typename T, int D, bool SLOPE, bool STATES_ONLY>
+template <typename T, int D, bool SLOPE, bool STATES_ONLY, bool WIDE>
 __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a, const int first_run)
 {
     using Sh = Shape<D>;
@@ -139,10 +151,10 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
     const int pad = (int)(chunks * C - len), reverse = r.reverse;
 
     if (!STATES_ONLY) {                                       // rows behind the sequence, dealt out over the segments
-        T* out = (T*)r.out + (((int64_t)b * a.steps + len) * a.heads + h) * F;
-        const int64_t n = (a.steps - len) * F;
-        for (int64_t i = (int64_t)seg * N + tid; i < n; i += (int64_t)a.segments * N)
-            out[i / F * a.heads * F + i % F] = pxg_from_f32<T>(0.f);
+        for (int64_t t = len + seg * Sh::waves + wave; t < a.steps; t += a.segments * Sh::waves) {
+            T* out = (T*)r.out + (((int64_t)b * a.steps + t) * a.heads + h) * F;
+            for (int f = lane; f < F; f += 64) out[f] = pxg_from_f32<T>(0.f);
+        }
     }
     if (STATES_ONLY && c_first + a.segment_chunks >= chunks) return;            // nothing behind it waits for its state
     if (c_first >= chunks && !(seg == 0 && chunks == 0)) {
@@ -156,6 +168,9 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
     __syncthreads();
     // factors of one lane: inside a diagonal tile, for tiles further off, for the state (index r: step 4 g + r of a tile)
     f32x4 w_diag, w_off, w_state;
+    float tiles[CT];                                          // and for whole tiles
+#pragma unroll
+    for (int n = 0; n < CT; n++) tiles[n] = pw[16 * n];
 #pragma unroll
     for (int s = 0; s < 4; s++) {
         const int d = li - 4 * g - s;
@@ -187,16 +202,25 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
     const T* const x = (const T*)r.x.data + b * r.x.batch_stride + h * r.x.head_stride;
     const T* const y = (const T*)r.y.data + b * r.y.batch_stride + h * r.y.head_stride;
     const T* const z = (const T*)r.z.data + b * r.z.batch_stride + h * r.z.head_stride;
+    // What is loaded for the next chunk stays in registers while this one is computed: the loads take no branch (rows in front of
+    // the sequence and columns behind the width read something that is there, and are cleared on their way to shared memory).
     Piece<T> px[STATES_ONLY ? 1 : PIECES], py[PIECES], pz[PIECES];
     const auto fetch = [&](int64_t c) {
 #pragma unroll
         for (int n = 0; n < PIECES; n++) {
             const int at = tid + n * N, col = at % (D / 8) * 8;
-            const int64_t u = c * C + at / (D / 8) - pad, t = reverse ? len - 1 - u : u;
-            const bool live = u >= 0;
-            py[n] = load_piece(y + t * r.y.step_stride, col, E, r.wide & 2, live);
-            pz[n] = load_piece(z + t * r.z.step_stride, col, F, r.wide & 4, live);
-            if constexpr (!STATES_ONLY) px[n] = load_piece(x + t * r.x.step_stride, col, E, r.wide & 1, live);
+            int64_t u = c * C + at / (D / 8) - pad;
+            u = u > 0 ? u : 0;
+            const int64_t t = reverse ? len - 1 - u : u;
+            if constexpr (WIDE) {
+                py[n] = load_wide(y + t * r.y.step_stride + (col < E ? col : 0));
+                pz[n] = load_wide(z + t * r.z.step_stride + (col < F ? col : 0));
+                if constexpr (!STATES_ONLY) px[n] = load_wide(x + t * r.x.step_stride + (col < E ? col : 0));
+            } else {
+                py[n] = load_narrow(y + t * r.y.step_stride, col, E);
+                pz[n] = load_narrow(z + t * r.z.step_stride, col, F);
+                if constexpr (!STATES_ONLY) px[n] = load_narrow(x + t * r.x.step_stride, col, E);
+            }
         }
     };
     const auto x_block = [&](int it, int k, int p) {          // x of steps it * 16 .., columns 32 k .. as an operand, permuted
@@ -217,7 +241,11 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
         bool fine = true;
 #pragma unroll
         for (int n = 0; n < PIECES; n++) {
-            const int at = tid + n * N, o = at / (D / 8) * ROW + at % (D / 8) * 8;
+            const int at = tid + n * N, col = at % (D / 8) * 8, o = at / (D / 8) * ROW + col;
+            const bool live = c > 0 || at / (D / 8) >= pad;
+            clear_unless(live && col < E, py[n]);
+            clear_unless(live && col < F, pz[n]);
+            if constexpr (!STATES_ONLY) clear_unless(live && col < E, px[n]);
             store_piece<T, PLANE>(py[n], ty + o);
             store_piece<T, PLANE>(pz[n], tz + o);
             if constexpr (!STATES_ONLY) {
@@ -300,7 +328,7 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
                                 for (int s = 0; s < 4; s++) acc[s] = li >= 4 * g + s ? acc[s] * w_diag[s] : 0.f;
                             } else {
                                 acc *= w_off;
-                                if (it - jt > 1) acc *= pw[16 * (it - jt - 1)];
+                                if (it - jt > 1) acc *= tiles[it - jt - 1];
                             }
                         }
                         weight[half] = acc;
@@ -340,6 +368,7 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
                         if (odd_values && k == it / 2) {
                             // one row of the tile at a time, without the z of the rows behind it
                             f32x4 sum = o[s], sum_slope = d[SLOPE ? s : 0];
+#pragma unroll 1
                             for (int i = 0; i < 16; i++) {
                                 bf16x8 zz[NP];
 #pragma unroll
@@ -368,7 +397,7 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
                     for (int s = 0; s < SL; s++) {
                         const int f = (wave * SL + s) * 16 + 4 * g;
                         T* out = (T*)r.out + row * F + f;
-                        if (r.wide & 16) {
+                        if constexpr (WIDE) {
                             if (f < F) {
                                 struct alignas(4 * sizeof(T)) Four { T v[4]; } four;
 #pragma unroll
@@ -384,7 +413,7 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
                             const T* q = (const T*)r.dot.data + b * r.dot.batch_stride + t * r.dot.step_stride + h * r.dot.head_stride + f;
 #pragma unroll
                             for (int k = 0; k < 4; k++)
-                                if (f + k < F) part = fmaf((float)q[k], d[s][k], part);
+                                if (WIDE ? f < F : f + k < F) part = fmaf((float)q[k], d[s][k], part);
                         }
                     }
                 }
@@ -414,7 +443,7 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
 #pragma unroll
                     for (int q = 1; q < NP; q++) value += __builtin_convertvector(read_transposed(at + q * PLANE), f32x4);
                     value *= w_state;
-                    if (jt < CT - 1) value *= pw[16 * (CT - 1 - jt)];
+                    if (jt < CT - 1) value *= tiles[CT - 1 - jt];
                     split<3>(value, u[half]);
                     if constexpr (SLOPE) {
 #pragma unroll
@@ -486,27 +515,35 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
     }
 }
 
-template <typename T, int D>
+template <typename T, int D, bool WIDE>
 int launch_width(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream)
 {
     const dim3 grid(a.batch * a.heads, states_only ? a.segments - 1 : a.segments, n), block(Shape<D>::threads);
     if (states_only) {
-        if (slope) k_chunks<T, D, true, true><<<grid, block, 0, stream>>>(a, first);
-        else k_chunks<T, D, false, true><<<grid, block, 0, stream>>>(a, first);
+        if (slope) k_chunks<T, D, true, true, WIDE><<<grid, block, 0, stream>>>(a, first);
+        else k_chunks<T, D, false, true, WIDE><<<grid, block, 0, stream>>>(a, first);
     } else {
-        if (slope) k_chunks<T, D, true, false><<<grid, block, 0, stream>>>(a, first);
-        else k_chunks<T, D, false, false><<<grid, block, 0, stream>>>(a, first);
+        if (slope) k_chunks<T, D, true, false, WIDE><<<grid, block, 0, stream>>>(a, first);
+        else k_chunks<T, D, false, false, WIDE><<<grid, block, 0, stream>>>(a, first);
     }
     return hipGetLastError() == hipSuccess ? PXG_OK : PXG_E_HIP;
+}
+
+template <typename T, int D> int launch_rows(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream)
+{
+    bool wide = true;
+    for (int i = first; i < first + n; i++) wide &= a.run[i].wide != 0;
+    return wide ? launch_width<T, D, true>(a, first, n, slope, states_only, stream)
+                : launch_width<T, D, false>(a, first, n, slope, states_only, stream);
 }
 
 template <typename T> int launch(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream)
 {
     switch (decay_width(a.run[first].E, a.run[first].F)) {
-    case 16: return launch_width<T, 16>(a, first, n, slope, states_only, stream);
-    case 32: return launch_width<T, 32>(a, first, n, slope, states_only, stream);
-    case 64: return launch_width<T, 64>(a, first, n, slope, states_only, stream);
-    default: return launch_width<T, 128>(a, first, n, slope, states_only, stream);
+    case 16: return launch_rows<T, 16>(a, first, n, slope, states_only, stream);
+    case 32: return launch_rows<T, 32>(a, first, n, slope, states_only, stream);
+    case 64: return launch_rows<T, 64>(a, first, n, slope, states_only, stream);
+    default: return launch_rows<T, 128>(a, first, n, slope, states_only, stream);
     }
 }
 
