@@ -158,7 +158,7 @@ bool wide(const pxg_sequence& s, int width, int dtype)
 
 void finish_run(DecayRun& r, int dtype)
 {
-    r.wide = wide(r.x, r.E, dtype) && wide(r.y, r.E, dtype) && wide(r.z, r.F, dtype) && (uintptr_t)r.out % 16 == 0;
+    r.wide = wide(r.x, r.E, dtype) && wide(r.y, r.E, dtype) && wide(r.z, r.F, dtype) && (!r.partial || wide(r.dot, r.F, dtype)) && (uintptr_t)r.out % 16 == 0;
 }
 
 }  // namespace
