@@ -148,12 +148,12 @@ DecayRuns runs_of(const pxg_decay* a, const Cut& c)
     return s;
 }
 
-// rows that can be read 16 bytes at a time, in whole groups of eight elements
+// rows that can be read 16 bytes at a time, in whole groups of eight elements, a chunk of them within 32 bits of one another
 bool wide(const pxg_sequence& s, int width, int dtype)
 {
     const int64_t unit = dtype == PXG_DT_F32 ? 4 : 8;
     return (uintptr_t)s.data % 16 == 0 && width % 8 == 0 && s.batch_stride % unit == 0 && s.step_stride % unit == 0 &&
-           s.head_stride % unit == 0;
+           s.head_stride % unit == 0 && s.step_stride >= 0 && s.step_stride < 1 << 24;
 }
 
 void finish_run(DecayRun& r, int dtype)

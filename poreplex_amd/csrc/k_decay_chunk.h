@@ -42,6 +42,11 @@ template <> struct Type<float> { static constexpr int planes = 3, code = PXG_DT_
 template <> struct Type<pxg_f16> { static constexpr int planes = 2, code = PXG_DT_F16; };
 template <> struct Type<pxg_bf16> { static constexpr int planes = 1, code = PXG_DT_BF16; };
 
+struct No { static constexpr bool value = false; };
+struct Yes { static constexpr bool value = true; };
+static constexpr No no;
+static constexpr Yes yes;
+
 template <int D> struct Shape {
     static constexpr int waves = D / 16, threads = 64 * waves;
     static constexpr int row = D + 8;                          // of shared memory: 16 bytes more, an odd number of 16-byte units
@@ -163,7 +168,7 @@ __device__ __forceinline__ int xcd_order(int id, int n)
 }
 
 template <typename T, int D, bool SLOPE, bool STATES_ONLY, bool WIDE>
-__global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a, const int first_run)
+__global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns a, const int first_run)
 {
     using Sh = Shape<D>;
     constexpr int NP = Type<T>::planes, C = decay_chunk(Type<T>::code, D), CT = C / 16, ET = Sh::et, KB = Sh::kb;
@@ -240,13 +245,35 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
         }
 
     // What is loaded for the next chunk stays in registers while this one is computed: the loads take no branch (rows in front of
-    // the sequence and columns behind the width read something that is there, and are cleared on their way to shared memory).
+    // the sequence and columns behind the width read something that is there, and are cleared on their way to shared memory).  From
+    // the second chunk on a lane's place in the chunk is a constant offset from its first step.
     const T* const x = (const T*)r.x.data + b * r.x.batch_stride + h * r.x.head_stride;
     const T* const y = (const T*)r.y.data + b * r.y.batch_stride + h * r.y.head_stride;
     const T* const z = (const T*)r.z.data + b * r.z.batch_stride + h * r.z.head_stride;
     const T* const q = DOT ? (const T*)r.dot.data + b * r.dot.batch_stride + h * r.dot.head_stride : nullptr;
     Piece<T> px[OUT ? PIECES : 1], py[PIECES], pz[PIECES], pq[DOT ? PIECES : 1];
+    uint32_t ox[PIECES], oy[PIECES], oz[PIECES], oq[PIECES];                    // in elements
+#pragma unroll
+    for (int n = 0; n < PIECES; n++) {
+        const int at = tid + n * N, col = at % (D / 8) * 8, row = reverse ? C - 1 - at / (D / 8) : at / (D / 8);
+        const uint32_t ce = col < E ? col : 0, cf = col < F ? col : 0;
+        ox[n] = row * (uint32_t)r.x.step_stride + ce, oy[n] = row * (uint32_t)r.y.step_stride + ce;
+        oz[n] = row * (uint32_t)r.z.step_stride + cf, oq[n] = DOT ? row * (uint32_t)r.dot.step_stride + cf : 0;
+    }
     const auto fetch = [&](int64_t c) {
+        if (WIDE && c > 0) {
+            const int64_t t = reverse ? len - (c + 1) * C + pad : c * C - pad;
+            const T *xs = x + t * r.x.step_stride, *ys = y + t * r.y.step_stride, *zs = z + t * r.z.step_stride;
+            const T* qs = DOT ? q + t * r.dot.step_stride : nullptr;
+#pragma unroll
+            for (int n = 0; n < PIECES; n++) {
+                py[n] = load_wide(ys + oy[n]);
+                pz[n] = load_wide(zs + oz[n]);
+                if constexpr (OUT) px[n] = load_wide(xs + ox[n]);
+                if constexpr (DOT) pq[n] = load_wide(qs + oq[n]);
+            }
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < PIECES; n++) {
             const int at = tid + n * N, col = at % (D / 8) * 8;
@@ -411,67 +438,80 @@ __global__ __launch_bounds__(Shape<D>::threads) void k_chunks(const DecayRuns a,
         if (!works) continue;
 
         if constexpr (OUT) {
+            // P z, 32 earlier steps at a time
+            const auto add_block = [&](int it, int k, auto careful) {
+                bf16x8 wp[KEEP + 1], zb[NP];
+#pragma unroll
+                for (int p = 0; p <= KEEP; p++) {
+                    const __bf16* at = weights + p * PPLANE + (it * 16 + li) * PROW + k * 32 + 4 * g;
+                    wp[p] = join(*(const bf16x4*)at, 2 * k + 1 <= it ? *(const bf16x4*)(at + 16) : bf16x4{});
+                }
+#pragma unroll
+                for (int n = 0; n < NP; n++) {
+                    const __bf16* at = tz + n * PLANE + k * 32 * ROW + f0 + at_tr;
+                    zb[n] = join(read_transposed(at), read_transposed(at + 16 * ROW));
+                }
+                const auto add = [&](const bf16x8* zz, f32x4 to) {
+#pragma unroll
+                    for (int p = KEEP; p >= 0; p--)
+#pragma unroll
+                        for (int n = 0; n < NP; n++)
+                            if (p + n <= KEEP) to = mfma(zz[n], wp[p], to);
+                    return to;
+                };
+                if constexpr (decltype(careful)::value) {
+                    // one row of the tile at a time, without the z of the rows behind it
+                    const f32x4 before = o[it];
+#pragma unroll 1
+                    for (int i = 0; i < 16; i++) {
+                        bf16x8 zz[NP];
+#pragma unroll
+                        for (int n = 0; n < NP; n++)
+#pragma unroll
+                            for (int m = 0; m < 8; m++) {
+                                const int j = (m / 4 - it % 2) * 16 + 4 * g + m % 4;             // from the tile's first row
+                                zz[n][m] = j <= i ? zb[n][m] : (__bf16)0.f;
+                            }
+                        const f32x4 one = add(zz, before);
+                        if (li == i) o[it] = one;
+                    }
+                } else {
+                    o[it] = add(zb, o[it]);
+                }
+            };
+            if (odd_values) {
+#pragma unroll
+                for (int it = 0; it < CT; it++) {
+#pragma unroll
+                    for (int k = 0; k < it / 2; k++) add_block(it, k, no);
+                    add_block(it, it / 2, yes);
+                }
+            } else {
+#pragma unroll
+                for (int it = 0; it < CT; it++)
+#pragma unroll
+                    for (int k = 0; k <= it / 2; k++) add_block(it, k, no);
+            }
+            // rows of the result: four columns of this lane's step
+            const int64_t first = reverse ? len - 1 - c * C + pad : c * C - pad;
+            T* const out = (T*)r.out + (((int64_t)b * a.steps + first) * a.heads + h) * F + f0 + 4 * g;
+            const int64_t out_step = (int64_t)(reverse ? -a.heads : a.heads) * F;
 #pragma unroll
             for (int it = 0; it < CT; it++) {
-#pragma unroll
-                for (int k = 0; k <= it / 2; k++) {           // 32 earlier steps at a time
-                    bf16x8 wp[KEEP + 1], zb[NP];
-#pragma unroll
-                    for (int p = 0; p <= KEEP; p++) {
-                        const __bf16* at = weights + p * PPLANE + (it * 16 + li) * PROW + k * 32 + 4 * g;
-                        wp[p] = join(*(const bf16x4*)at, 2 * k + 1 <= it ? *(const bf16x4*)(at + 16) : bf16x4{});
-                    }
-#pragma unroll
-                    for (int n = 0; n < NP; n++) {
-                        const __bf16* at = tz + n * PLANE + k * 32 * ROW + f0 + at_tr;
-                        zb[n] = join(read_transposed(at), read_transposed(at + 16 * ROW));
-                    }
-                    const auto add = [&](const bf16x8* zz, f32x4 to) {
-#pragma unroll
-                        for (int p = KEEP; p >= 0; p--)
-#pragma unroll
-                            for (int n = 0; n < NP; n++)
-                                if (p + n <= KEEP) to = mfma(zz[n], wp[p], to);
-                        return to;
-                    };
-                    if (odd_values && k == it / 2) {
-                        // one row of the tile at a time, without the z of the rows behind it
-                        f32x4 sum = o[it];
-#pragma unroll 1
-                        for (int i = 0; i < 16; i++) {
-                            bf16x8 zz[NP];
-#pragma unroll
-                            for (int n = 0; n < NP; n++)
-#pragma unroll
-                                for (int m = 0; m < 8; m++) {
-                                    const int j = (m / 4 - it % 2) * 16 + 4 * g + m % 4;         // from the tile's first row
-                                    zz[n][m] = j <= i ? zb[n][m] : (__bf16)0.f;
-                                }
-                            const f32x4 one = add(zz, o[it]);
-                            if (li == i) sum = one;
-                        }
-                        o[it] = sum;
-                    } else {
-                        o[it] = add(zb, o[it]);
-                    }
-                }
-                // rows of the result: four columns of this lane's step
-                const int64_t u = c * C + it * 16 + li - pad, t = reverse ? len - 1 - u : u;
+                if (c == 0 && it * 16 + li < pad) continue;
+                T* const at = out + (it * 16 + li) * out_step;
                 const int f = f0 + 4 * g;
-                if (u >= 0) {
-                    T* out = (T*)r.out + (((int64_t)b * a.steps + t) * a.heads + h) * F + f;
-                    if constexpr (WIDE) {
-                        if (f < F) {
-                            struct alignas(4 * sizeof(T)) Four { T v[4]; } four;
+                if constexpr (WIDE) {
+                    if (f < F) {
+                        struct alignas(4 * sizeof(T)) Four { T v[4]; } four;
 #pragma unroll
-                            for (int k = 0; k < 4; k++) four.v[k] = pxg_from_f32<T>(o[it][k]);
-                            *(Four*)out = four;
-                        }
-                    } else {
-#pragma unroll
-                        for (int k = 0; k < 4; k++)
-                            if (f + k < F) out[k] = pxg_from_f32<T>(o[it][k]);
+                        for (int k = 0; k < 4; k++) four.v[k] = pxg_from_f32<T>(o[it][k]);
+                        *(Four*)at = four;
                     }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        if (f + k < F) at[k] = pxg_from_f32<T>(o[it][k]);
                 }
             }
         }
