@@ -39,10 +39,7 @@ __device__ __forceinline__ int64_t decay_length(const DecayRuns& s, int b)
 // steps in a chunk, by the type's number of bfloat16 planes and the padded width
 constexpr int decay_chunk(int dtype, int width)
 {
-#ifdef CH
-    return CH;
-#endif
-    return (dtype == PXG_DT_BF16 && width > 32) || (dtype == PXG_DT_F16 && width == 64) ? 64 : 32;
+    return 32;
 }
 constexpr int decay_width(int e, int f)
 {

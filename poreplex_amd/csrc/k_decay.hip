@@ -16,6 +16,8 @@ namespace {
 
 // carry[s] becomes the state in front of segment s + 1: each segment's own, plus what came before it, decayed over its length;
 // the slopes behind the states decay and grow with the distance.
+constexpr int AT_ONCE = 8;
+
 __global__ __launch_bounds__(256) void k_decay_join(const DecayRuns a, int chunk, int slope_runs)
 {
     const DecayRun& r = a.run[blockIdx.z];
@@ -27,11 +29,24 @@ __global__ __launch_bounds__(256) void k_decay_join(const DecayRuns a, int chunk
     const float steps = (float)a.segment_chunks * (float)chunk, decay = expf(steps * a.log_decay[bh % a.heads]);
     const bool slope = (int)blockIdx.z < slope_runs;
     float* c = r.carry + bh * n * size + i;
+    const int64_t last = used > 0 ? (used - 1) / a.segment_chunks : 0;         // the last segment with chunks: states 0 .. last - 1 are read
     float S = c[0], G = slope ? c[slopes] : 0.f;
-    for (int64_t s = 1; s < n && (s + 1) * a.segment_chunks < used; s++) {
-        c += size;
-        if (slope) c[slopes] = G = fmaf(decay, G + steps * S, c[slopes]);
-        *c = S = fmaf(decay, S, *c);
+    for (int64_t s = 1; s < last; s += AT_ONCE) {                              // the loads of some, then the chain through them
+        float own[AT_ONCE], own_slope[AT_ONCE];
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++) {
+            if (s + j >= last) break;
+            own[j] = c[(s + j) * size];
+            own_slope[j] = slope ? c[slopes + (s + j) * size] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < AT_ONCE; j++) {
+            if (s + j >= last) break;
+            G = fmaf(decay, G + steps * S, own_slope[j]);
+            S = fmaf(decay, S, own[j]);
+            c[(s + j) * size] = S;
+            if (slope) c[slopes + (s + j) * size] = G;
+        }
     }
 }
 
@@ -116,18 +131,25 @@ bool bad_operands(const pxg_decay* a)
     return !a->log_decay || (any && (!a->q.data || !a->k.data || !a->v.data));
 }
 
-// How the time axis is cut: not at all where (sequence, head) pairs alone fill the card, else into enough segments that do, of at
-// least four chunks each.  What the segments cost is a second reading of y and z.
+// How the time axis is cut.  The cost of segments is a second reading of y and z, their gain waves that hide each other's latency:
+// a pass takes them where its (sequence, head) pairs come to no more than 1 024 waves (four for each CU), and enough of them for
+// 4 096 (forward) or 2 048 (backward, which has three runs to do), of at least four chunks each (eight where that fills a quarter
+// of the card by itself: 1 024 pairs x 300 steps x 16 wide f32 31 -> 47).  Forward / backward in us, uncut
+// and cut: 128 pairs x 2 000 steps x 64 wide bf16 113 / 263 -> 61 / 190, 256 pairs (the limit) 113 / 287 -> 98 / 293, 384 pairs
+// 129 / 361 -> 146 / 475; 256 pairs x 16 wide f32 (one wave each) 171 / 418 -> 71 / 201.
 struct Cut {
     int segments, chunks;
 };
 
-Cut cut_of(const pxg_decay* a)
+Cut cut_of(const pxg_decay* a, bool backward)
 {
-    const int64_t chunk = decay_chunk(a->dtype, decay_width(a->dk, a->dv)), chunks = (a->steps + chunk - 1) / chunk;
-    const int64_t pairs = a->batch * a->heads;
-    int64_t segments = pairs < 256 && pairs > 0 ? (512 + pairs - 1) / pairs : 1;
-    if (segments > chunks / 4) segments = chunks / 4;
+    const int width = decay_width(a->dk, a->dv);
+    const int64_t chunk = decay_chunk(a->dtype, width), chunks = (a->steps + chunk - 1) / chunk;
+    const int64_t waves = a->batch * a->heads * (width / 16);
+    int64_t segments = 1;
+    if (waves > 0 && waves <= (backward ? 1023 : 1024)) segments = ((backward ? 2048 : 4096) + waves - 1) / waves;
+    const int64_t least = waves > 256 ? 8 : 4;                 // chunks of a segment
+    if (segments > chunks / least) segments = chunks / least;
     if (segments < 1) segments = 1;
     const int64_t each = segments > 1 ? (chunks + segments - 1) / segments : chunks > 0 ? chunks : 1;
     Cut c = {(int)(segments > 1 ? (chunks + each - 1) / each : 1), (int)each};
@@ -166,7 +188,7 @@ void finish_run(DecayRun& r, int dtype)
 extern "C" int64_t pxg_decay_workspace_bytes(const pxg_decay* a, int32_t backward)
 {
     if (bad_shape(a)) return PXG_E_INVALID;
-    const Cut c = cut_of(a);
+    const Cut c = cut_of(a, backward != 0);
     // the states between segments (backward: of three runs, and the slopes of one), the partial sums of grad_log_decay
     return (int64_t)sizeof(float) * (carry_values(a, c) * (backward ? 4 : 1) + (backward ? a->batch * a->heads * c.segments : 0));
 }
@@ -178,7 +200,7 @@ extern "C" int pxg_decay_forward(const pxg_decay* a, void* stream)
     if (a->steps > 0 && !a->out) return PXG_E_INVALID;
     const int64_t bytes = pxg_decay_workspace_bytes(a, 0);
     if (a->workspace_bytes < bytes || (bytes > 0 && !a->workspace)) return PXG_E_INVALID;
-    DecayRuns s = runs_of(a, cut_of(a));
+    DecayRuns s = runs_of(a, cut_of(a, false));
     DecayRun& r = s.run[0];
     r.x = a->q, r.y = a->k, r.z = a->v;
     r.init = a->initial_state, r.fin = a->final_state, r.init_e = a->dv, r.init_f = 1;
@@ -196,7 +218,7 @@ extern "C" int pxg_decay_backward(const pxg_decay* a, void* stream)
     const int64_t bytes = pxg_decay_workspace_bytes(a, 1);
     if (a->workspace_bytes < bytes || (bytes > 0 && !a->workspace)) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
-    const Cut c = cut_of(a);
+    const Cut c = cut_of(a, true);
     DecayRuns s = runs_of(a, c);
     float* const partial = (float*)a->workspace + 4 * carry_values(a, c);
     int rc = PXG_OK;

@@ -167,27 +167,32 @@ __device__ __forceinline__ int xcd_order(int id, int n)
     return x * each + (x < more ? x : more) + id / 8;
 }
 
+// waves of a SIMD that the registers are to leave room for
+constexpr int waves_wanted(int planes, int width, bool slope, bool states_only)
+{
+    if (states_only) return 3;
+    if (slope || (planes == 3 && (width == 16 || width == 128))) return 2;
+    return planes == 2 && width == 128 ? 4 : 3;
+}
+
 template <typename T, int D, bool SLOPE, bool STATES_ONLY, bool WIDE>
-__global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns a, const int first_run)
+__global__ __launch_bounds__(Shape<D>::threads, waves_wanted(Type<T>::planes, D, SLOPE, STATES_ONLY))
+void k_chunks(const DecayRuns a, const int first_run)
 {
     using Sh = Shape<D>;
     constexpr int NP = Type<T>::planes, C = decay_chunk(Type<T>::code, D), CT = C / 16, ET = Sh::et, KB = Sh::kb;
     constexpr int ROW = Sh::row, PLANE = C * ROW, N = Sh::threads, W = Sh::waves, PIECES = C * (D / 8) / N;
     constexpr int KEEP = NP == 3 ? 2 : 1;                     // products of planes p + q <= KEEP go into the result
     constexpr int PROW = C + 8, PPLANE = C * PROW;            // of the weights
-    constexpr int SLOPE_PLANES = NP == 3 ? 3 : 2;
+    constexpr int SLOPE_PLANES = 3;
     constexpr bool OUT = !STATES_ONLY, DOT = SLOPE && OUT;
     static_assert(PIECES * N == C * (D / 8), "whole pieces");
-    __shared__ __attribute__((aligned(16))) __bf16 tile[(OUT ? DOT ? 4 : 3 : 2) * NP * PLANE];
+    constexpr int ROWS = (OUT ? DOT ? 4 : 3 : 2) * NP * PLANE;
+    __shared__ __attribute__((aligned(16))) __bf16 tile[ROWS];
     __shared__ __attribute__((aligned(16))) __bf16 weights[OUT ? (KEEP + 1) * PPLANE : 8];
     __shared__ float pw[C + 1];
     __shared__ int strange[2];
-    __bf16* const ty = tile;
-    __bf16* const tz = tile + NP * PLANE;
-    __bf16* const tx = tile + (OUT ? 2 * NP * PLANE : 0);
-    __bf16* const tq = tile + (DOT ? 3 * NP * PLANE : 0);
-
-    const DecayRun& r = a.run[first_run + blockIdx.z];
+    const DecayRun r = a.run[first_run + blockIdx.z];
     const int bh = xcd_order(blockIdx.x, gridDim.x), b = bh / a.heads, h = bh % a.heads, seg = blockIdx.y;
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, g = lane / 16, li = lane % 16, f0 = wave * 16;
     const int E = r.E, F = r.F;
@@ -231,18 +236,30 @@ __global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns
     const bool from_carry = seg > 0 && OUT;
     const int64_t at_carry = ((int64_t)bh * (a.segments - 1) + seg - 1) * E * F;
     const int64_t slopes = (int64_t)a.batch * a.heads * (a.segments - 1) * E * F;
+    const float* const start = from_carry ? r.carry + at_carry : seg == 0 && r.init ? r.init + base : nullptr;
+    const int start_e = from_carry ? F : (int)r.init_e, start_f = from_carry ? 1 : (int)r.init_f;
 #pragma unroll
-    for (int t = 0; t < ET; t++)
+    for (int t = 0; t < ET; t++) {
+        S[t] = f32x4{};
+        if constexpr (SLOPE) G[t] = f32x4{};
+    }
+    if (start) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int e = t * 16 + 4 * g + k, f = f0 + li;
-            const bool in = e < E && f < F;
-            float v = 0.f;
-            if (in && from_carry) v = r.carry[at_carry + e * F + f];
-            else if (in && seg == 0 && r.init) v = r.init[base + e * r.init_e + f * r.init_f];
-            S[t][k] = v;
-            if constexpr (SLOPE) G[t][k] = in && from_carry ? r.carry[slopes + at_carry + e * F + f] : 0.f;
-        }
+        for (int t = 0; t < ET; t++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const int e = t * 16 + 4 * g + k, f = f0 + li;
+                const bool in = e < E && f < F;
+                const int at = in ? e * start_e + f * start_f : 0;
+                const float v = start[at];
+                S[t][k] = in ? v : 0.f;
+                if constexpr (SLOPE)
+                    if (from_carry) {
+                        const float w = start[slopes + at];
+                        G[t][k] = in ? w : 0.f;
+                    }
+            }
+    }
 
     // What is loaded for the next chunk stays in registers while this one is computed: the loads take no branch (rows in front of
     // the sequence and columns behind the width read something that is there, and are cleared on their way to shared memory).  From
@@ -261,19 +278,6 @@ __global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns
         oz[n] = row * (uint32_t)r.z.step_stride + cf, oq[n] = DOT ? row * (uint32_t)r.dot.step_stride + cf : 0;
     }
     const auto fetch = [&](int64_t c) {
-        if (WIDE && c > 0) {
-            const int64_t t = reverse ? len - (c + 1) * C + pad : c * C - pad;
-            const T *xs = x + t * r.x.step_stride, *ys = y + t * r.y.step_stride, *zs = z + t * r.z.step_stride;
-            const T* qs = DOT ? q + t * r.dot.step_stride : nullptr;
-#pragma unroll
-            for (int n = 0; n < PIECES; n++) {
-                py[n] = load_wide(ys + oy[n]);
-                pz[n] = load_wide(zs + oz[n]);
-                if constexpr (OUT) px[n] = load_wide(xs + ox[n]);
-                if constexpr (DOT) pq[n] = load_wide(qs + oq[n]);
-            }
-            return;
-        }
 #pragma unroll
         for (int n = 0; n < PIECES; n++) {
             const int at = tid + n * N, col = at % (D / 8) * 8;
@@ -292,6 +296,22 @@ __global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns
                 if constexpr (OUT) px[n] = load_narrow(x + t * r.x.step_stride, col, E);
                 if constexpr (DOT) pq[n] = load_narrow(q + t * r.dot.step_stride, col, F);
             }
+        }
+    };
+    const auto fetch_next = [&](int64_t c) {
+        if constexpr (WIDE) {
+            const int64_t t = reverse ? len - (c + 1) * C + pad : c * C - pad;
+            const T *xs = x + t * r.x.step_stride, *ys = y + t * r.y.step_stride, *zs = z + t * r.z.step_stride;
+            const T* qs = DOT ? q + t * r.dot.step_stride : nullptr;
+#pragma unroll
+            for (int n = 0; n < PIECES; n++) {
+                py[n] = load_wide(ys + oy[n]);
+                pz[n] = load_wide(zs + oz[n]);
+                if constexpr (OUT) px[n] = load_wide(xs + ox[n]);
+                if constexpr (DOT) pq[n] = load_wide(qs + oq[n]);
+            }
+        } else {
+            fetch(c);
         }
     };
     // steps 16 n .. of a tile, columns 32 k .. as an operand, permuted
@@ -315,14 +335,12 @@ __global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns
         }
         return acc;
     };
+    __bf16 *const ty = tile, *const tz = tile + NP * PLANE, *const tx = tile + (OUT ? 2 * NP * PLANE : 0), *const tq = tile + (DOT ? 3 * NP * PLANE : 0);
     const int at_tr = (4 * g + li / 4) * ROW + li % 4 * 4;    // of a lane in a 16 x 16 block that is read transposed
     const bool narrow = E < D || F < D;
     float part = 0.f;
 
-    if (c_first < c_last) fetch(c_first);
-    for (int64_t c = c_first; c < c_last; c++) {
-        const int odd = (int)(c & 1);
-        __syncthreads();
+    const auto stage = [&](int64_t c) {                       // what was fetched, into shared memory
         if (narrow || c == 0) {
 #pragma unroll
             for (int n = 0; n < PIECES; n++) {
@@ -338,17 +356,26 @@ __global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns
 #pragma unroll
         for (int n = 0; n < PIECES; n++) {
             const int at = tid + n * N, o = at / (D / 8) * ROW + at % (D / 8) * 8;
-            store_piece<T, PLANE>(py[n], ty + o);
-            store_piece<T, PLANE>(pz[n], tz + o);
+            store_piece<T, PLANE>(py[n], tile + o);
+            store_piece<T, PLANE>(pz[n], tile + NP * PLANE + o);
             if constexpr (OUT) {
-                store_piece<T, PLANE>(px[n], tx + o);
+                store_piece<T, PLANE>(px[n], tile + 2 * NP * PLANE + o);
                 most = magnitude(pz[n], most);
             }
-            if constexpr (DOT) store_piece<T, PLANE>(pq[n], tq + o);
+            if constexpr (DOT) store_piece<T, PLANE>(pq[n], tile + 3 * NP * PLANE + o);
         }
-        if (OUT && !finite_magnitude<T>(most)) strange[odd] = 1;
-        if (c + 1 < c_last) fetch(c + 1);
-        __syncthreads();
+        if (OUT && !finite_magnitude<T>(most)) strange[c & 1] = 1;
+    };
+
+    if (c_first < c_last) {
+        fetch(c_first);
+        stage(c_first);
+    }
+    __builtin_amdgcn_s_waitcnt(0x0f70);                       // the state is there (vmcnt 0): no wait for it, and the rows behind it, in the loop
+    for (int64_t c = c_first; c < c_last; c++) {
+        __syncthreads();                                      // the chunk's rows are there
+        if (c + 1 < c_last) fetch_next(c + 1);
+        if (tid == 0) strange[(c + 1) & 1] = 0;
         const int skip = c == 0 ? pad + (reverse && seg == 0 ? 1 : 0) : 0;      // steps by which the state's decay is short
 
         if constexpr (OUT) {
@@ -432,12 +459,64 @@ __global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns
                 o[it] *= w;
             }
         }
-        if constexpr (OUT) __syncthreads();
-        const bool odd_values = OUT && strange[odd];
-        if (tid == 0) strange[odd ^ 1] = 0;
-        if (!works) continue;
-
-        if constexpr (OUT) {
+        if (works) {
+            // the state behind the chunk
+            const float decay = pw[C - skip];
+#pragma unroll
+            for (int t = 0; t < ET; t++) {
+                if constexpr (SLOPE) G[t] = (G[t] + S[t] * (float)(C - skip)) * decay;
+                S[t] *= decay;
+            }
+#pragma unroll
+            for (int k = 0; k < C / 32; k++) {
+                bf16x8 zw[3], zs[SLOPE ? SLOPE_PLANES : 1];
+                bf16x4 u[2][3], v[2][SLOPE ? SLOPE_PLANES : 1];
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    const int jt = 2 * k + half;
+                    const __bf16* at = tz + jt * 16 * ROW + f0 + at_tr;
+                    f32x4 value = widen(read_transposed(at + (NP - 1) * PLANE));
+#pragma unroll
+                    for (int n = NP - 2; n >= 0; n--) value += widen(read_transposed(at + n * PLANE));
+                    value *= w_state;
+                    if (jt < CT - 1) value *= tiles[CT - 1 - jt];
+                    split<3>(value, u[half]);
+                    if constexpr (SLOPE) {
+#pragma unroll
+                        for (int n = 0; n < 4; n++) value[n] *= (float)(C - 1 - jt * 16 - 4 * g - n);
+                        split<SLOPE_PLANES>(value, v[half]);
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < 3; p++) zw[p] = join(u[0][p], u[1][p]);
+                if constexpr (SLOPE)
+#pragma unroll
+                    for (int p = 0; p < SLOPE_PLANES; p++) zs[p] = join(v[0][p], v[1][p]);
+#pragma unroll
+                for (int t = 0; t < ET; t++) {
+                    bf16x8 yt[NP];
+#pragma unroll
+                    for (int n = 0; n < NP; n++) {
+                        const __bf16* at = ty + n * PLANE + k * 32 * ROW + t * 16 + at_tr;
+                        yt[n] = join(read_transposed(at), read_transposed(at + 16 * ROW));
+                    }
+#pragma unroll
+                    for (int p = 2; p >= 0; p--)
+#pragma unroll
+                        for (int n = 0; n < NP; n++)
+                            if (p + n <= 2) S[t] = mfma(yt[n], zw[p], S[t]);
+                    if constexpr (SLOPE) {
+#pragma unroll
+                        for (int p = SLOPE_PLANES - 1; p >= 0; p--)
+#pragma unroll
+                            for (int n = 0; n < NP; n++)
+                                if (p + n < SLOPE_PLANES) G[t] = mfma(yt[n], zs[p], G[t]);
+                    }
+                }
+            }
+        }
+        if constexpr (OUT) __syncthreads();                   // the weights are there
+        if (OUT && works) {
             // P z, 32 earlier steps at a time
             const auto add_block = [&](int it, int k, auto careful) {
                 bf16x8 wp[KEEP + 1], zb[NP];
@@ -479,7 +558,7 @@ __global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns
                     o[it] = add(zb, o[it]);
                 }
             };
-            if (odd_values) {
+            if (strange[c & 1]) {
 #pragma unroll
                 for (int it = 0; it < CT; it++) {
 #pragma unroll
@@ -492,13 +571,16 @@ __global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns
 #pragma unroll
                     for (int k = 0; k <= it / 2; k++) add_block(it, k, no);
             }
+        }
+        const auto write = [&] {
+            if (!OUT || !works) return;
             // rows of the result: four columns of this lane's step
             const int64_t first = reverse ? len - 1 - c * C + pad : c * C - pad;
             T* const out = (T*)r.out + (((int64_t)b * a.steps + first) * a.heads + h) * F + f0 + 4 * g;
             const int64_t out_step = (int64_t)(reverse ? -a.heads : a.heads) * F;
 #pragma unroll
             for (int it = 0; it < CT; it++) {
-                if (c == 0 && it * 16 + li < pad) continue;
+                if (c == 0 && it * 16 + li < pad) continue;   // in front of the sequence
                 T* const at = out + (it * 16 + li) * out_step;
                 const int f = f0 + 4 * g;
                 if constexpr (WIDE) {
@@ -514,84 +596,48 @@ __global__ __launch_bounds__(Shape<D>::threads, 2) void k_chunks(const DecayRuns
                         if (f + k < F) at[k] = pxg_from_f32<T>(o[it][k]);
                 }
             }
+        };
+        if (c + 1 == c_last) {
+            write();
+            break;
         }
-
-        // the state behind the chunk
-        const float decay = pw[C - skip];
-#pragma unroll
-        for (int t = 0; t < ET; t++) {
-            if constexpr (SLOPE) G[t] = (G[t] + S[t] * (float)(C - skip)) * decay;
-            S[t] *= decay;
-        }
-#pragma unroll
-        for (int k = 0; k < C / 32; k++) {
-            bf16x8 zw[3], zs[SLOPE ? SLOPE_PLANES : 1];
-            bf16x4 u[2][3], v[2][SLOPE ? SLOPE_PLANES : 1];
-#pragma unroll
-            for (int half = 0; half < 2; half++) {
-                const int jt = 2 * k + half;
-                const __bf16* at = tz + jt * 16 * ROW + f0 + at_tr;
-                f32x4 value = widen(read_transposed(at + (NP - 1) * PLANE));
-#pragma unroll
-                for (int n = NP - 2; n >= 0; n--) value += widen(read_transposed(at + n * PLANE));
-                value *= w_state;
-                if (jt < CT - 1) value *= tiles[CT - 1 - jt];
-                split<3>(value, u[half]);
-                if constexpr (SLOPE) {
-#pragma unroll
-                    for (int n = 0; n < 4; n++) value[n] *= (float)(C - 1 - jt * 16 - 4 * g - n);
-                    split<SLOPE_PLANES>(value, v[half]);
-                }
-            }
-#pragma unroll
-            for (int p = 0; p < 3; p++) zw[p] = join(u[0][p], u[1][p]);
-            if constexpr (SLOPE)
-#pragma unroll
-                for (int p = 0; p < SLOPE_PLANES; p++) zs[p] = join(v[0][p], v[1][p]);
-#pragma unroll
-            for (int t = 0; t < ET; t++) {
-                bf16x8 yt[NP];
-#pragma unroll
-                for (int n = 0; n < NP; n++) {
-                    const __bf16* at = ty + n * PLANE + k * 32 * ROW + t * 16 + at_tr;
-                    yt[n] = join(read_transposed(at), read_transposed(at + 16 * ROW));
-                }
-#pragma unroll
-                for (int p = 2; p >= 0; p--)
-#pragma unroll
-                    for (int n = 0; n < NP; n++)
-                        if (p + n <= 2) S[t] = mfma(yt[n], zw[p], S[t]);
-                if constexpr (SLOPE) {
-#pragma unroll
-                    for (int p = SLOPE_PLANES - 1; p >= 0; p--)
-#pragma unroll
-                        for (int n = 0; n < NP; n++)
-                            if (p + n < SLOPE_PLANES) G[t] = mfma(yt[n], zs[p], G[t]);
-                }
-            }
-        }
+        // staged before the stores: the wait for what was fetched is no wait for them
+        __syncthreads();
+        stage(c + 1);
+        write();
     }
 
     // where the state goes: to the next segment, or behind the sequence
     const bool last = c_last == chunks;
     const int64_t to_carry = ((int64_t)bh * (a.segments - 1) + seg) * E * F;
     const float end = reverse && len > 0 ? pw[1] : 1.f;       // S before the first step is the gradient's a R
+    float* const fin = STATES_ONLY ? r.carry + to_carry : last && r.fin ? r.fin + base : nullptr;
+    const int fin_e = STATES_ONLY ? F : (int)r.init_e, fin_f = STATES_ONLY ? 1 : (int)r.init_f;
+    if (fin) {
 #pragma unroll
-    for (int t = 0; t < ET; t++)
+        for (int t = 0; t < ET; t++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const int e = t * 16 + 4 * g + k, f = f0 + li;
-            if (e >= E || f >= F) continue;
-            if constexpr (STATES_ONLY) {
-                r.carry[to_carry + e * F + f] = S[t][k];
-                if constexpr (SLOPE) r.carry[slopes + to_carry + e * F + f] = G[t][k];
-            } else if (last) {
-                const int64_t at = base + e * r.init_e + f * r.init_f;
-                if (r.fin) r.fin[at] = end * S[t][k];
-                if constexpr (SLOPE)
-                    if (r.grad_fin) part = fmaf(r.grad_fin[at], G[t][k], part);
+            for (int k = 0; k < 4; k++) {
+                const int e = t * 16 + 4 * g + k, f = f0 + li;
+                if (e < E && f < F) {
+                    fin[e * fin_e + f * fin_f] = STATES_ONLY ? S[t][k] : end * S[t][k];
+                    if constexpr (STATES_ONLY && SLOPE) fin[slopes + e * fin_e + f * fin_f] = G[t][k];
+                }
             }
+    }
+    if constexpr (DOT) {
+        if (last && r.grad_fin) {
+#pragma unroll
+            for (int t = 0; t < ET; t++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int e = t * 16 + 4 * g + k, f = f0 + li;
+                    const bool in = e < E && f < F;
+                    const float v = r.grad_fin[base + (in ? e * (int)r.init_e + f * (int)r.init_f : 0)];
+                    part = fmaf(in ? v : 0.f, G[t][k], part);
+                }
         }
+    }
     if constexpr (DOT) {
 #pragma unroll
         for (int m = 32; m; m >>= 1) part += __shfl_xor(part, m);
