@@ -16,7 +16,7 @@ struct DecayRun {
     // gradient of log_decay (the run of dq): q's rows, the gradient of the final state, one partial sum per (batch * heads, segment)
     pxg_sequence dot;
     const float* grad_fin;
-    float* partial;
+    double* partial;
 };
 
 struct DecayRuns {

@@ -25,38 +25,38 @@ __global__ __launch_bounds__(256) void k_decay_join(const DecayRuns a, int chunk
     const int64_t slopes = (int64_t)a.batch * a.heads * n * size;
     const int i = blockIdx.y * 256 + threadIdx.x;
     if (i >= size) return;
-    const int64_t len = decay_length(a, (int)(bh / a.heads)), used = (len + chunk - 1) / chunk;
-    const float steps = (float)a.segment_chunks * (float)chunk, decay = expf(steps * a.log_decay[bh % a.heads]);
+    const int used = (int)((uint32_t)(decay_length(a, (int)bh / a.heads) + chunk - 1) / (uint32_t)chunk);
+    const float steps = (float)a.segment_chunks * (float)chunk, decay = expf(steps * a.log_decay[(int)bh % a.heads]);
     const bool slope = (int)blockIdx.z < slope_runs;
     float* c = r.carry + bh * n * size + i;
-    const int64_t last = used > 0 ? (used - 1) / a.segment_chunks : 0;         // the last segment with chunks: states 0 .. last - 1 are read
     float S = c[0], G = slope ? c[slopes] : 0.f;
-    for (int64_t s = 1; s < last; s += AT_ONCE) {                              // the loads of some, then the chain through them
+    // state s is read by segment s + 1, if that has chunks
+    const auto needed = [&](int s) { return s < n && (s + 1) * a.segment_chunks < used; };
+    for (int s = 1; needed(s); s += AT_ONCE) {                                 // the loads of some, then the chain through them
         float own[AT_ONCE], own_slope[AT_ONCE];
 #pragma unroll
         for (int j = 0; j < AT_ONCE; j++) {
-            if (s + j >= last) break;
-            own[j] = c[(s + j) * size];
-            own_slope[j] = slope ? c[slopes + (s + j) * size] : 0.f;
+            own[j] = needed(s + j) ? c[(s + j) * size] : 0.f;
+            own_slope[j] = slope && needed(s + j) ? c[slopes + (s + j) * size] : 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < AT_ONCE; j++) {
-            if (s + j >= last) break;
-            G = fmaf(decay, G + steps * S, own_slope[j]);
-            S = fmaf(decay, S, own[j]);
-            c[(s + j) * size] = S;
-            if (slope) c[slopes + (s + j) * size] = G;
-        }
+        for (int j = 0; j < AT_ONCE; j++)
+            if (needed(s + j)) {
+                G = fmaf(decay, G + steps * S, own_slope[j]);
+                S = fmaf(decay, S, own[j]);
+                c[(s + j) * size] = S;
+                if (slope) c[slopes + (s + j) * size] = G;
+            }
     }
 }
 
 // grad_log_decay[h] = the sum of the partial sums [batch][heads][segments], in a fixed order
-__global__ __launch_bounds__(256) void k_decay_sum(const float* partial, int64_t batch, int heads, int segments, float* out)
+__global__ __launch_bounds__(256) void k_decay_sum(const double* partial, int64_t batch, int heads, int segments, float* out)
 {
     __shared__ double red[256];
     double sum = 0.0;
     for (int64_t i = threadIdx.x; i < batch * segments; i += 256)
-        sum += (double)partial[(i / segments * heads + blockIdx.x) * segments + i % segments];
+        sum += partial[(i / segments * heads + blockIdx.x) * segments + i % segments];
     red[threadIdx.x] = sum;
     __syncthreads();
     for (int w = 128; w; w >>= 1) {
@@ -92,29 +92,96 @@ int launch_runs(const DecayRuns& a, int dtype, int n, int slope_runs, hipStream_
     return rc;
 }
 
-// One step: the state is read once and written once, which is all the time this takes.
-template <typename T>
-__global__ __launch_bounds__(128) void k_decay_step(pxg_decay a)
+// One step.  The state is read once and written once, 8 dk dv bytes for 5 dk dv operations: bandwidth is all there is.  P threads
+// have a (sequence, head) pair, each four columns of every (4 P / columns)-th row, four rows in flight; their parts of o meet in
+// shared memory.  A pair of up to 32 x 32 takes a wave (four of them a workgroup, so that small states fill a CU), a larger one a
+// workgroup.
+template <typename T, int P>
+__global__ __launch_bounds__(256) void k_decay_step(const pxg_decay a)
 {
-    const int f = threadIdx.x, b = blockIdx.x / a.heads, h = blockIdx.x % a.heads;
-    if (f >= a.dv) return;
-    T* out = (T*)a.out + (int64_t)blockIdx.x * a.dv;
-    if (a.lengths && !((const uint8_t*)a.lengths)[b]) {
-        out[f] = pxg_from_f32<T>(0.f);
-        return;
+    constexpr int PAIRS = 256 / P, ROWS = 4;
+    __shared__ float qs[PAIRS][PXG_DECAY_MAX_WIDTH], ks[PAIRS][PXG_DECAY_MAX_WIDTH];
+    __shared__ __attribute__((aligned(16))) float parts[PAIRS][P][4];
+    const int own = threadIdx.x / P, t = threadIdx.x % P, dk = a.dk, dv = a.dv;
+    const int64_t pairs = a.batch * a.heads, pair = (int64_t)blockIdx.x * PAIRS + own;
+    const bool there = pair < pairs;
+    const int64_t b = there ? pair / a.heads : 0, h = there ? pair % a.heads : 0;
+    const bool active = there && !(a.lengths && !((const uint8_t*)a.lengths)[b]);
+    const int groups = (dv + 3) / 4, every = P / groups, col = t % groups * 4, first = t / groups;       // groups <= 32 <= P
+    const bool works = active && first < every;
+    float* const S = a.final_state + (there ? pair : 0) * dk * dv + col;
+    const bool wide = dv % 4 == 0 && (uintptr_t)a.final_state % 16 == 0;
+    const auto load = [&](int e) {
+        float4 s = {};
+        if (wide) s = *(const float4*)(S + e * dv);
+        else {
+            s.x = S[e * dv];
+            if (col + 1 < dv) s.y = S[e * dv + 1];
+            if (col + 2 < dv) s.z = S[e * dv + 2];
+            if (col + 3 < dv) s.w = S[e * dv + 3];
+        }
+        return s;
+    };
+    float4 s[ROWS];
+    if (works)
+#pragma unroll
+        for (int n = 0; n < ROWS; n++)
+            if (first + n * every < dk) s[n] = load(first + n * every);
+    if (active) {
+        const T* q = (const T*)a.q.data + b * a.q.batch_stride + h * a.q.head_stride;
+        const T* k = (const T*)a.k.data + b * a.k.batch_stride + h * a.k.head_stride;
+        for (int e = t; e < dk; e += P) qs[own][e] = pxg_to_f32(q[e]), ks[own][e] = pxg_to_f32(k[e]);
     }
-    const T* q = (const T*)a.q.data + b * a.q.batch_stride + h * a.q.head_stride;
-    const T* k = (const T*)a.k.data + b * a.k.batch_stride + h * a.k.head_stride;
-    const float v = pxg_to_f32(((const T*)a.v.data + b * a.v.batch_stride + h * a.v.head_stride)[f]);
-    float* S = a.final_state + (int64_t)blockIdx.x * a.dk * a.dv + f;
-    const float decay = expf(a.log_decay[h]);
-    float o = 0.f;
-    for (int e = 0; e < a.dk; e++, S += a.dv) {
-        const float now = fmaf(decay, *S, pxg_to_f32(k[e]) * v);
-        *S = now;
-        o = fmaf(pxg_to_f32(q[e]), now, o);
+    float v[4] = {}, o[4] = {};
+    float decay = 0.f;
+    if (works) {
+        const T* at = (const T*)a.v.data + b * a.v.batch_stride + h * a.v.head_stride + col;
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+            if (col + n < dv) v[n] = pxg_to_f32(at[n]);
+        decay = expf(a.log_decay[h]);
     }
-    out[f] = pxg_from_f32<T>(o);
+    __syncthreads();
+    if (works)
+        for (int e0 = first; e0 < dk; e0 += ROWS * every) {
+            float4 next[ROWS];
+#pragma unroll
+            for (int n = 0; n < ROWS; n++)
+                if (e0 + (n + ROWS) * every < dk) next[n] = load(e0 + (n + ROWS) * every);
+#pragma unroll
+            for (int n = 0; n < ROWS; n++) {
+                const int e = e0 + n * every;
+                if (e >= dk) break;
+                const float ke = ks[own][e], qe = qs[own][e];
+                const float4 now = {fmaf(decay, s[n].x, ke * v[0]), fmaf(decay, s[n].y, ke * v[1]), fmaf(decay, s[n].z, ke * v[2]),
+                                    fmaf(decay, s[n].w, ke * v[3])};
+                if (wide) *(float4*)(S + e * dv) = now;
+                else {
+                    S[e * dv] = now.x;
+                    if (col + 1 < dv) S[e * dv + 1] = now.y;
+                    if (col + 2 < dv) S[e * dv + 2] = now.z;
+                    if (col + 3 < dv) S[e * dv + 3] = now.w;
+                }
+                o[0] = fmaf(qe, now.x, o[0]), o[1] = fmaf(qe, now.y, o[1]), o[2] = fmaf(qe, now.z, o[2]), o[3] = fmaf(qe, now.w, o[3]);
+            }
+#pragma unroll
+            for (int n = 0; n < ROWS; n++) s[n] = next[n];
+        }
+    *(float4*)parts[own][t] = float4{o[0], o[1], o[2], o[3]};
+    __syncthreads();
+    if (there)
+        for (int f = t; f < dv; f += P) {
+            float sum = 0.f;
+            for (int n = 0; n < every; n++) sum += parts[own][n * groups + f / 4][f % 4];
+            ((T*)a.out)[pair * dv + f] = pxg_from_f32<T>(active ? sum : 0.f);
+        }
+}
+
+template <typename T> void launch_step(const pxg_decay& a, hipStream_t stream)
+{
+    const int64_t pairs = a.batch * a.heads;
+    if ((int64_t)a.dk * a.dv <= 1024) k_decay_step<T, 64><<<(unsigned)((pairs + 3) / 4), 256, 0, stream>>>(a);
+    else k_decay_step<T, 256><<<(unsigned)pairs, 256, 0, stream>>>(a);
 }
 
 bool bad_shape(const pxg_decay* a)
@@ -190,7 +257,8 @@ extern "C" int64_t pxg_decay_workspace_bytes(const pxg_decay* a, int32_t backwar
     if (bad_shape(a)) return PXG_E_INVALID;
     const Cut c = cut_of(a, backward != 0);
     // the states between segments (backward: of three runs, and the slopes of one), the partial sums of grad_log_decay
-    return (int64_t)sizeof(float) * (carry_values(a, c) * (backward ? 4 : 1) + (backward ? a->batch * a->heads * c.segments : 0));
+    return backward ? (int64_t)sizeof(double) * a->batch * a->heads * c.segments + (int64_t)sizeof(float) * 4 * carry_values(a, c)
+                    : (int64_t)sizeof(float) * carry_values(a, c);
 }
 
 extern "C" int pxg_decay_forward(const pxg_decay* a, void* stream)
@@ -220,7 +288,7 @@ extern "C" int pxg_decay_backward(const pxg_decay* a, void* stream)
     hipStream_t st = (hipStream_t)stream;
     const Cut c = cut_of(a, true);
     DecayRuns s = runs_of(a, c);
-    float* const partial = (float*)a->workspace + 4 * carry_values(a, c);
+    double* const partial = (double*)a->workspace;
     int rc = PXG_OK;
     if (a->batch > 0) {
         DecayRun &dq = s.run[0], &dk = s.run[1], &dv = s.run[2];
@@ -234,7 +302,7 @@ extern "C" int pxg_decay_backward(const pxg_decay* a, void* stream)
         dv.x = a->k, dv.y = a->q, dv.z = a->grad_out, dv.reverse = 1;
         dv.init = a->grad_final_state, dv.fin = a->grad_initial_state, dv.init_e = a->dv, dv.init_f = 1;
         dv.out = a->grad_v, dv.E = a->dk, dv.F = a->dv;
-        dq.carry = (float*)a->workspace;                                      // states and slopes
+        dq.carry = (float*)(partial + a->batch * a->heads * c.segments);                                      // states and slopes
         dk.carry = dq.carry + 2 * carry_values(a, c), dv.carry = dk.carry + carry_values(a, c);
         for (DecayRun& r : s.run) finish_run(r, a->dtype);
         rc = launch_runs(s, a->dtype, 3, a->grad_log_decay ? 1 : 0, st);
@@ -251,12 +319,11 @@ extern "C" int pxg_decay_step(const pxg_decay* a, void* stream)
     if (bad_shape(a) || a->steps != 1 || bad_operands(a)) return PXG_E_INVALID;
     if (a->batch == 0) return PXG_OK;
     if (!a->out || !a->final_state) return PXG_E_INVALID;
-    const int blocks = (int)a->batch * a->heads;
     hipStream_t st = (hipStream_t)stream;
     switch (a->dtype) {
-    case PXG_DT_F32: k_decay_step<float><<<blocks, 128, 0, st>>>(*a); break;
-    case PXG_DT_BF16: k_decay_step<pxg_bf16><<<blocks, 128, 0, st>>>(*a); break;
-    default: k_decay_step<pxg_f16><<<blocks, 128, 0, st>>>(*a);
+    case PXG_DT_F32: launch_step<float>(*a, st); break;
+    case PXG_DT_BF16: launch_step<pxg_bf16>(*a, st); break;
+    default: launch_step<pxg_f16>(*a, st);
     }
     return hipGetLastError() == hipSuccess ? PXG_OK : PXG_E_HIP;
 }

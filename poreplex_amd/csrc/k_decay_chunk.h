@@ -29,6 +29,7 @@
 // a chunk that has one takes its diagonal products row by row, with later rows' z left out.
 #pragma once
 #include "k_decay.h"
+#include <type_traits>
 
 namespace decay {
 
@@ -71,6 +72,33 @@ __device__ __forceinline__ f32x4 widen(bf16x4 v)
 {
     const uint2 u = __builtin_bit_cast(uint2, v);
     return f32x4{low_of(u.x), high_of(u.x), low_of(u.y), high_of(u.y)};
+}
+
+// Products of planes, the small ones first.  Heads of 16 fill half of an instruction's k axis: two products share one.
+template <int NU, int NV, int LIMIT> __device__ __forceinline__ f32x4 plane_products(const bf16x8* u, const bf16x8* v, f32x4 acc)
+{
+#pragma unroll
+    for (int p = NU - 1; p >= 0; p--)
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+            if (p + n <= LIMIT) acc = mfma(u[p], v[n], acc);
+    return acc;
+}
+template <int NU, int NV, int LIMIT> __device__ __forceinline__ f32x4 plane_products(const bf16x4* u, const bf16x4* v, f32x4 acc)
+{
+    bf16x4 wait_u = {}, wait_v = {};
+    bool waits = false;
+#pragma unroll
+    for (int p = NU - 1; p >= 0; p--)
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+            if (p + n <= LIMIT) {
+                if (waits) acc = mfma(join(wait_u, u[p]), join(wait_v, v[n]), acc);
+                else wait_u = u[p], wait_v = v[n];
+                waits = !waits;
+            }
+    if (waits) acc = mfma(join(wait_u, bf16x4{}), join(wait_v, bf16x4{}), acc);
+    return acc;
 }
 
 // four floats into N planes, the largest part first
@@ -210,7 +238,7 @@ void k_chunks(const DecayRuns a, const int first_run)
     }
     if (STATES_ONLY && c_first + a.segment_chunks >= chunks) return;            // nothing behind it waits for its state
     if (c_first >= chunks && !(seg == 0 && chunks == 0)) {
-        if (SLOPE && tid == 0) r.partial[(int64_t)bh * a.segments + seg] = 0.f;
+        if (SLOPE && tid == 0) r.partial[(int64_t)bh * a.segments + seg] = 0.0;
         return;
     }
 
@@ -314,31 +342,30 @@ void k_chunks(const DecayRuns a, const int first_run)
             fetch(c);
         }
     };
-    // steps 16 n .. of a tile, columns 32 k .. as an operand, permuted
+    // steps 16 n .. of a tile, columns 32 k .. as an operand, permuted (heads of 16: half an operand)
+    using Operand = std::conditional_t<D == 16, bf16x4, bf16x8>;
     const auto block = [&](const __bf16* of, int n, int k, int p) {
         const __bf16* at = of + p * PLANE + (n * 16 + li) * ROW + k * 32 + 4 * g;
-        return join(*(const bf16x4*)at, D == 16 ? bf16x4{} : *(const bf16x4*)(at + (D == 16 ? 0 : 16)));
+        if constexpr (D == 16) return *(const bf16x4*)at;
+        else return join(*(const bf16x4*)at, *(const bf16x4*)(at + 16));
     };
     // x_i . y_j, transposed, for tiles n and m of 16 steps
     const auto products = [&](const __bf16* of_j, const __bf16* of_i, int m, int n) {
         f32x4 acc = {};
 #pragma unroll
         for (int k = 0; k < KB; k++) {
-            bf16x8 u[NP], v[NP];
+            Operand u[NP], v[NP];
 #pragma unroll
             for (int p = 0; p < NP; p++) u[p] = block(of_j, m, k, p), v[p] = block(of_i, n, k, p);
-#pragma unroll
-            for (int p = NP - 1; p >= 0; p--)
-#pragma unroll
-                for (int o = 0; o < NP; o++)
-                    if (p + o <= 2) acc = mfma(u[p], v[o], acc);
+            acc = plane_products<NP, NP, 2>(u, v, acc);
         }
         return acc;
     };
     __bf16 *const ty = tile, *const tz = tile + NP * PLANE, *const tx = tile + (OUT ? 2 * NP * PLANE : 0), *const tq = tile + (DOT ? 3 * NP * PLANE : 0);
     const int at_tr = (4 * g + li / 4) * ROW + li % 4 * 4;    // of a lane in a 16 x 16 block that is read transposed
     const bool narrow = E < D || F < D;
-    float part = 0.f;
+    float part = 0.f;                                         // of one chunk; `total` of all
+    double total = 0.0;
 
     const auto stage = [&](int64_t c) {                       // what was fetched, into shared memory
         if (narrow || c == 0) {
@@ -380,7 +407,11 @@ void k_chunks(const DecayRuns a, const int first_run)
 
         if constexpr (OUT) {
             // the weights, each wave its tiles
-            for (int n = wave; n < CT * (CT + 1) / 2; n += W) {
+            constexpr int TILES = CT * (CT + 1) / 2;
+#pragma unroll
+            for (int turn = 0; turn < (TILES + W - 1) / W; turn++) {
+                const int n = W == 1 ? turn : wave + turn * W;
+                if (n >= TILES) break;
                 const int it = n < 1 ? 0 : n < 3 ? 1 : n < 6 ? 2 : 3, jt = n - it * (it + 1) / 2;
                 f32x4 acc = products(ty, tx, jt, it);
                 if (it == jt) {
@@ -417,30 +448,29 @@ void k_chunks(const DecayRuns a, const int first_run)
             }
 #pragma unroll
             for (int k = 0; k < KB; k++) {
-                bf16x4 u[KEEP + 1], v[KEEP + 1] = {}, gu[SLOPE ? SLOPE_PLANES : 1], gv[SLOPE ? SLOPE_PLANES : 1] = {};
-                split<KEEP + 1>(S[2 * k], u);
-                if constexpr (D > 16) split<KEEP + 1>(S[2 * k + 1], v);
-                if constexpr (DOT) {
-                    split<SLOPE_PLANES>(G[2 * k], gu);
-                    if constexpr (D > 16) split<SLOPE_PLANES>(G[2 * k + 1], gv);
-                }
+                Operand su[KEEP + 1], gu[SLOPE ? SLOPE_PLANES : 1];
+                const auto operand = [&](const f32x4* of, auto planes, Operand* to) {
+                    constexpr int M = decltype(planes)::value;
+                    bf16x4 u[M], v[M];
+                    split<M>(of[D == 16 ? 0 : 2 * k], u);
+                    if constexpr (D > 16) {
+                        split<M>(of[2 * k + 1], v);
+#pragma unroll
+                        for (int p = 0; p < M; p++) to[p] = join(u[p], v[p]);
+                    } else {
+#pragma unroll
+                        for (int p = 0; p < M; p++) to[p] = u[p];
+                    }
+                };
+                operand(S, std::integral_constant<int, KEEP + 1>(), su);
+                if constexpr (DOT) operand(G, std::integral_constant<int, SLOPE_PLANES>(), gu);
 #pragma unroll
                 for (int it = 0; it < CT; it++) {
-                    bf16x8 xb[NP];
+                    Operand xb[NP];
 #pragma unroll
                     for (int p = 0; p < NP; p++) xb[p] = block(tx, it, k, p);
-#pragma unroll
-                    for (int p = KEEP; p >= 0; p--)
-#pragma unroll
-                        for (int n = 0; n < NP; n++)
-                            if (p + n <= KEEP) o[it] = mfma(join(u[p], v[p]), xb[n], o[it]);
-                    if constexpr (DOT) {
-#pragma unroll
-                        for (int p = SLOPE_PLANES - 1; p >= 0; p--)
-#pragma unroll
-                            for (int n = 0; n < NP; n++)
-                                if (p + n < SLOPE_PLANES) d[it] = mfma(join(gu[p], gv[p]), xb[n], d[it]);
-                    }
+                    o[it] = plane_products<KEEP + 1, NP, KEEP>(su, xb, o[it]);
+                    if constexpr (DOT) d[it] = plane_products<SLOPE_PLANES, NP, SLOPE_PLANES - 1>(gu, xb, d[it]);
                 }
             }
 #pragma unroll
@@ -572,6 +602,7 @@ void k_chunks(const DecayRuns a, const int first_run)
                     for (int k = 0; k <= it / 2; k++) add_block(it, k, no);
             }
         }
+        if constexpr (DOT) total += (double)part, part = 0.f;
         const auto write = [&] {
             if (!OUT || !works) return;
             // rows of the result: four columns of this lane's step
@@ -639,14 +670,15 @@ void k_chunks(const DecayRuns a, const int first_run)
         }
     }
     if constexpr (DOT) {
+        total += (double)part;
 #pragma unroll
-        for (int m = 32; m; m >>= 1) part += __shfl_xor(part, m);
-        __syncthreads();
-        if (lane == 0) pw[wave] = part;
+        for (int m = 32; m; m >>= 1) total += __shfl_xor(total, m);
+        __shared__ double sums[W];
+        if (lane == 0) sums[wave] = total;
         __syncthreads();
         if (tid == 0) {
-            float sum = 0.f;
-            for (int i = 0; i < W; i++) sum += pw[i];
+            double sum = 0.0;
+            for (int i = 0; i < W; i++) sum += sums[i];
             r.partial[(int64_t)bh * a.segments + seg] = sum;
         }
     }

@@ -62,7 +62,7 @@ __device__ __forceinline__ float value_of(uint32_t key)
 }
 
 // exp((x - base) / temperature): the factor log2(e) / temperature as a sum of two floats, so that the exponent of a far
-// element is off by its own rounding only
+// element is off by its own rounding only.  Of half-precision rows one float is enough: they are off by more themselves.
 struct Scale {
     float hi, lo;
 };
@@ -76,9 +76,10 @@ __device__ __forceinline__ Scale scale_of(float temperature)
     return s;
 }
 
-__device__ __forceinline__ float exp_from(float x, float base, Scale s)
+template <typename T> __device__ __forceinline__ float exp_from(float x, float base, Scale s)
 {
     const float d = x - base;                   // may be -inf: not times a number that may be 0 or below
+    if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(d * s.hi);
     return __builtin_amdgcn_exp2f(fmaf(d, s.hi, __builtin_amdgcn_fmed3f(d, -1e30f, 1e30f) * s.lo));
 }
 
@@ -88,36 +89,55 @@ template <typename T> struct Unit {
     T v[n];
 };
 
+template <typename T> __device__ __forceinline__ Unit<T> load_whole(const T* x, int64_t unit)
+{
+    Unit<T> u;
+    __builtin_memcpy(&u, x + unit * Unit<T>::n, sizeof u);
+    return u;
+}
+
 template <typename T> __device__ __forceinline__ Unit<T> load_unit(const T* x, int64_t unit, int64_t classes)
 {
     constexpr int n = Unit<T>::n;
+    if ((unit + 1) * n <= classes) return load_whole(x, unit);
     Unit<T> u;
-    if ((unit + 1) * n <= classes) {
-        __builtin_memcpy(&u, x + unit * n, sizeof u);
-    } else {
 #pragma unroll
-        for (int e = 0; e < n; e++) u.v[e] = unit * n + e < classes ? x[unit * n + e] : (T)-INFINITY;
-    }
+    for (int e = 0; e < n; e++) u.v[e] = unit * n + e < classes ? x[unit * n + e] : (T)-INFINITY;
     return u;
+}
+
+// Calls f(units, first unit, step) for this thread's units of a row, AHEAD at a time and step apart, as long as all of them are
+// whole (loads without a branch between them, so that all are on their way at once), then g(unit, its number) for those that are
+// left, the last of which may be cut.
+template <int G, typename T, typename F, typename L>
+__device__ __forceinline__ void each_units(const T* x, int64_t classes, int t, F f, L g)
+{
+    constexpr int n = Unit<T>::n;
+    const int64_t whole = classes / n, units = (classes + n - 1) / n;
+    int64_t i = t;
+    for (; i - t + G * AHEAD <= whole; i += G * AHEAD) {
+        Unit<T> u[AHEAD];
+#pragma unroll
+        for (int a = 0; a < AHEAD; a++) u[a] = load_whole(x, i + a * G);
+        f(u, i);
+    }
+    for (; i < units; i += G) g(load_unit(x, i, classes), i);
 }
 
 // calls f(first class, floats) for the units of a row that are this thread's
 template <int G, typename T, typename F> __device__ __forceinline__ void each_unit(const T* x, int64_t classes, int t, F f)
 {
     constexpr int n = Unit<T>::n;
-    const int64_t units = (classes + n - 1) / n;
-    for (int64_t i = t; i < units; i += G * AHEAD) {
-        Unit<T> u[AHEAD];
+    const auto one = [&](const Unit<T>& u, int64_t unit) {
+        float v[n];
 #pragma unroll
-        for (int a = 0; a < AHEAD; a++) u[a] = load_unit(x, i + a * G, classes);
+        for (int e = 0; e < n; e++) v[e] = pxg_to_f32(u.v[e]);
+        f(unit * n, v);
+    };
+    each_units<G>(x, classes, t, [&](const Unit<T>* u, int64_t unit) {
 #pragma unroll
-        for (int a = 0; a < AHEAD; a++) {
-            float v[n];
-#pragma unroll
-            for (int e = 0; e < n; e++) v[e] = pxg_to_f32(u[a].v[e]);
-            if (i + a * G < units) f((i + a * G) * n, v);
-        }
-    }
+        for (int a = 0; a < AHEAD; a++) one(u[a], unit + a * G);
+    }, one);
 }
 
 // ---- the largest logits ---------------------------------------------------------------------------------------------------------
@@ -185,11 +205,21 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
     float bound = value_of(bound_key), most = -INFINITY, sum = 0.f, base = __builtin_isfinite(bound) ? bound : 0.f;
     // everything below the bound: its largest element, and its sum against the bound
     each_unit<G>(x, classes, t, [&](int64_t first, const float* v) {
+        float here = v[0];
+        bool below = v[0] < bound;
+#pragma unroll
+        for (int e = 1; e < n; e++) here = fmaxf(here, v[e]), below &= v[e] < bound;
+        if (below) {                            // nearly every unit
+            most = fmaxf(most, here);
+#pragma unroll
+            for (int e = 0; e < n; e++) sum += exp_from<T>(v[e], base, scale);
+            return;
+        }
 #pragma unroll
         for (int e = 0; e < n; e++) {
             if (v[e] < bound) {
                 most = fmaxf(most, v[e]);
-                sum += exp_from(v[e], base, scale);
+                sum += exp_from<T>(v[e], base, scale);
             } else if (first + e < classes) {
                 const int at = atomicAdd(&s.count, 1);
                 if (at < CAND) s.cand[at] = (unsigned long long)order_of(v[e]) << 32 | (uint32_t)~(uint32_t)(first + e);
@@ -253,7 +283,7 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
                 for (int e = 0; e < n; e++) {
                     const uint32_t o = order_of(v[e]);
                     if (o < bound_key || (by_bisection && o == bound_key && (uint32_t)(first + e) >= before))
-                        sum += exp_from(v[e], base, scale);
+                        sum += exp_from<T>(v[e], base, scale);
                 }
             });
     }
@@ -437,35 +467,43 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_forward(const pxg
     // the student's unlisted classes: running maximum and sum
     const Scale scale = scale_of(a.temperature);
     float base_u = -3.402823466e38f, sum_u = 0.f;
-    {
-        const int64_t units = (a.classes + n - 1) / n;
-        for (int64_t i = t; i < units; i += G * AHEAD) {
-            Unit<T> u[AHEAD];
-            float v[AHEAD][n], next = base_u;
+    const auto numbers = [&](const Unit<T>& u, int64_t unit, float* v) {
+        const uint32_t mask = s.marks.of((int32_t)unit);
 #pragma unroll
-            for (int b = 0; b < AHEAD; b++) u[b] = load_unit(x, i + b * G, a.classes);
+        for (int e = 0; e < n; e++) v[e] = pxg_to_f32(u.v[e]);
+        if (mask)
 #pragma unroll
-            for (int b = 0; b < AHEAD; b++) {
-                const uint32_t mask = i + b * G < units ? s.marks.of((int32_t)(i + b * G)) : 0;
+            for (int e = 0; e < n; e++)
+                if (mask >> e & 1) v[e] = -INFINITY;
+    };
+    const auto raise = [&](float most) {                          // the sum's maximum
+        if (most > base_u) sum_u *= exp_from<T>(base_u, most, scale), base_u = most;
+    };
+    each_units<G>(x, a.classes, t, [&](const Unit<T>* u, int64_t unit) {
+        float v[AHEAD][n], next = base_u;
 #pragma unroll
-                for (int e = 0; e < n; e++) v[b][e] = pxg_to_f32(u[b].v[e]);
-                if (mask)
+        for (int b = 0; b < AHEAD; b++) {
+            numbers(u[b], unit + b * G, v[b]);
 #pragma unroll
-                    for (int e = 0; e < n; e++)
-                        if (mask >> e & 1) v[b][e] = -INFINITY;
-#pragma unroll
-                for (int e = 0; e < n; e++) next = fmaxf(next, v[b][e]);
-            }
-            if (next > base_u) sum_u *= exp_from(base_u, next, scale), base_u = next;
-#pragma unroll
-            for (int b = 0; b < AHEAD; b++)
-#pragma unroll
-                for (int e = 0; e < n; e++) sum_u += exp_from(v[b][e], base_u, scale);
+            for (int e = 0; e < n; e++) next = fmaxf(next, v[b][e]);
         }
-    }
+        raise(next);
+#pragma unroll
+        for (int b = 0; b < AHEAD; b++)
+#pragma unroll
+            for (int e = 0; e < n; e++) sum_u += exp_from<T>(v[b][e], base_u, scale);
+    }, [&](const Unit<T>& u, int64_t unit) {
+        float v[n], next = base_u;
+        numbers(u, unit, v);
+#pragma unroll
+        for (int e = 0; e < n; e++) next = fmaxf(next, v[e]);
+        raise(next);
+#pragma unroll
+        for (int e = 0; e < n; e++) sum_u += exp_from<T>(v[e], base_u, scale);
+    });
     const float all_u = group_reduce<G>(base_u, s.redf, MaxOf());
     // (a thread without any keeps its sum of 0 whatever its exponent says)
-    const double unlisted = group_reduce<G>(sum_u == 0.f ? 0.0 : (double)sum_u * (double)exp_from(base_u, all_u, scale), s.redd, SumOf());
+    const double unlisted = group_reduce<G>(sum_u == 0.f ? 0.0 : (double)sum_u * (double)exp_from<T>(base_u, all_u, scale), s.redd, SumOf());
 
     // the k + 1 shares
     double xi[PLACES], base = -INFINITY;
@@ -543,35 +581,35 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_backward(const px
         }
         group_sync<G>();
     }
-    const int64_t units = (a.classes + n - 1) / n;
-    for (int64_t i = t; i < units; i += G * AHEAD) {
-        Unit<T> u[AHEAD];
-        if (counts != 0.f) {
+    if (counts == 0.f) {
+        const int64_t units = (a.classes + n - 1) / n;
+        Unit<T> zero;
 #pragma unroll
-            for (int b = 0; b < AHEAD; b++) u[b] = load_unit(x, i + b * G, a.classes);
+        for (int e = 0; e < n; e++) zero.v[e] = pxg_from_f32<T>(0.f);
+        for (int64_t i = t; i < units; i += G) {
+            if ((i + 1) * n <= a.classes) __builtin_memcpy(g + i * n, &zero, sizeof zero);
+            else
+                for (int64_t v = i * n; v < a.classes; v++) g[v] = pxg_from_f32<T>(0.f);
         }
-#pragma unroll
-        for (int b = 0; b < AHEAD; b++) {
-            const int64_t unit = i + b * G;
-            if (unit >= units) continue;
-            uint32_t mask = 0;
-            if (counts != 0.f) {
-                mask = marks.of((int32_t)unit);
-#pragma unroll
-                for (int e = 0; e < n; e++) u[b].v[e] = pxg_from_f32<T>(exp_from(pxg_to_f32(u[b].v[e]), base_u, scale) * fc);
-            } else {
-#pragma unroll
-                for (int e = 0; e < n; e++) u[b].v[e] = pxg_from_f32<T>(0.f);
-            }
-            if (mask == 0 && (unit + 1) * n <= a.classes) {
-                __builtin_memcpy(g + unit * n, &u[b], sizeof u[b]);
-            } else {
-#pragma unroll
-                for (int e = 0; e < n; e++)
-                    if (!(mask >> e & 1) && unit * n + e < a.classes) g[unit * n + e] = u[b].v[e];
-            }
-        }
+        return;
     }
+    const auto one = [&](const Unit<T>& u, int64_t unit) {
+        Unit<T> r;
+#pragma unroll
+        for (int e = 0; e < n; e++) r.v[e] = pxg_from_f32<T>(exp_from<T>(pxg_to_f32(u.v[e]), base_u, scale) * fc);
+        const uint32_t mask = marks.of((int32_t)unit);
+        if (mask == 0 && (unit + 1) * n <= a.classes) {
+            __builtin_memcpy(g + unit * n, &r, sizeof r);
+        } else {
+#pragma unroll
+            for (int e = 0; e < n; e++)
+                if (!(mask >> e & 1) && unit * n + e < a.classes) g[unit * n + e] = r.v[e];
+        }
+    };
+    each_units<G>(x, a.classes, t, [&](const Unit<T>* u, int64_t unit) {
+#pragma unroll
+        for (int b = 0; b < AHEAD; b++) one(u[b], unit + b * G);
+    }, one);
 }
 
 // The threads that share a row: a wave for short ones, a workgroup of four waves, sixteen where there are too few rows to fill
