@@ -163,23 +163,24 @@ template <int G, typename T, typename F> __device__ __forceinline__ void each_un
 
 // ---- the largest logits ---------------------------------------------------------------------------------------------------------
 // One pass.  Each of the threads knows the largest of its own elements so far; the k-th largest of these 64 to 256 maxima is a bound
-// that at least k elements reach, and only so many more of evenly spread ones (k = 128 of 256: 177).  Elements below the bound are
-// added to the sum of the rest at once; the others become candidates.  The bound is raised as the row goes by, at the first tiles of
-// 4 units a thread and then ever more rarely, so that a row of any length has some hundred candidates.  They are ranked by counting;
-// what is not chosen joins the sum.  Rows with more than CAND (plateaus of equal values, rows that only ascend) take their bound by
-// bisection instead, reading the row again and again.
-//   2 047 x 50 001 bf16, k = 64: reading it a second time for the sum, from whatever cache has it, took 101 us, keeping it in
-//   registers (which leaves room for few workgroups) 222.
+// that at least k elements reach, and only so many more of evenly spread ones (k = 128 of 256: 177).  The bound is raised as the row
+// goes by, at the first tiles of 4 units a thread and then ever more rarely.  A unit below the bound is added to the sum of the rest
+// at once; the number of any other is noted, some hundred of them in a row of any length.  These are looked at again with the last
+// bound: what reaches it is ranked by counting, and all but the first k join the sum.  Rows with more than these lists hold (plateaus
+// of equal values, rows that only ascend) take their bound by bisection instead, reading the row again and again.
+//   2 047 x 50 001 bf16, k = 64: reading the row a second time for the sum, from whatever cache has it, took 101 us, keeping it in
+//   registers (which leaves room for few workgroups) 222, collecting elements instead of units' numbers 88.
 constexpr int CAND = 1024;
 
 template <int G> struct alignas(16) TopShared {
-    static constexpr int parts = G < 256 ? G : 256;
+    static constexpr int parts = G < 256 ? G : 256, notes = G == 64 ? 256 : 2048;       // G = 64: up to 256 units
     unsigned long long cand[CAND];              // (order, ~class): no two are equal
     uint32_t most[parts];
     double redd[G / 64];
     float redf[G / 64];
     int red[G / 64];
-    int count;
+    uint32_t note[notes];
+    int count, noted;
     uint32_t bound;
 };
 
@@ -196,7 +197,7 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
     const int t = threadIdx.x % G;
     const T* x = logits + row * row_stride;
     const Scale scale = scale_of<T>(temperature);
-    if (t == 0) s.count = 0;
+    if (t == 0) s.count = s.noted = 0;
 
     float largest = -INFINITY, bound = 0.f;
     const auto raise_bound = [&] {              // the k-th largest of the threads' maxima
@@ -224,31 +225,21 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
         bound = value_of(s.bound);
     };
     RunningSum<T> sum;
-    const auto take = [&](const float (&v)[n], int64_t first) {
+    const auto take = [&](const float (&v)[n], int64_t unit) {
         float here = v[0];
 #pragma unroll
         for (int e = 1; e < n; e++) here = larger(here, v[e]);
         if (here < bound) {                     // nearly every unit
             sum.add(v, here, scale);
-            return;
+        } else if (unit * n < classes) {
+            const int at = atomicAdd(&s.noted, 1);
+            if (at < TopShared<G>::notes) s.note[at] = (uint32_t)unit;
         }
-        float below[n], most = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < n; e++) {
-            const bool is = v[e] < bound;
-            below[e] = is ? v[e] : -INFINITY;
-            most = fmaxf(most, below[e]);
-            if (!is && first + e < classes) {
-                const int at = atomicAdd(&s.count, 1);
-                if (at < CAND) s.cand[at] = (unsigned long long)order_of(v[e]) << 32 | (uint32_t)~(uint32_t)(first + e);
-            }
-        }
-        sum.add(below, most, scale);
     };
     if (classes < (int64_t)G * n) {             // one element after the other: min(G, classes) threads have some, k at least
         for (int64_t v = t; v < classes; v += G) largest = larger(largest, pxg_to_f32(x[v]));
         raise_bound();
-        each_unit<G>(x, classes, t, [&](int64_t first, const float (&v)[n]) { take(v, first); });
+        each_unit<G>(x, classes, t, [&](int64_t first, const float (&v)[n]) { take(v, first / n); });
     } else {
         constexpr int64_t TILE = G * AHEAD;
         const int64_t whole = classes / n, units = (classes + n - 1) / n;
@@ -282,12 +273,33 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
             for (int a = 0; a < AHEAD; a++) {
                 float v[n];
                 numbers(u[a], v);
-                take(v, (i + a * G) * n);
+                take(v, i + a * G);
             }
         }
     }
+    if (classes >= (int64_t)G * n) raise_bound();
     group_sync<G>();
-    int found = s.count;
+    const int noted = s.noted;
+    if (noted <= TopShared<G>::notes)
+        for (int i = t; i < noted; i += G) {
+            const int64_t unit = s.note[i];
+            const Unit<T> u = load_unit(x, unit, classes);
+            float below[n], most = -INFINITY;
+#pragma unroll
+            for (int e = 0; e < n; e++) {
+                const float v = pxg_to_f32(u.v[e]);
+                const bool is = v < bound;
+                below[e] = is ? v : -INFINITY;
+                most = fmaxf(most, below[e]);
+                if (!is && unit * n + e < classes) {
+                    const int at = atomicAdd(&s.count, 1);
+                    if (at < CAND) s.cand[at] = (unsigned long long)order_of(v) << 32 | (uint32_t)~(uint32_t)(unit * n + e);
+                }
+            }
+            sum.add(below, most, scale);
+        }
+    group_sync<G>();
+    int found = noted <= TopShared<G>::notes ? s.count : CAND + 1;
     bool no_number = false;                     // among the rest (bisection only: otherwise it is a candidate)
     if (found > CAND) {
         // the largest key that k elements reach, bit by bit; then the smallest class below which enough of the ties lie
