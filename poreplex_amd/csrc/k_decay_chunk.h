@@ -217,7 +217,8 @@ void k_chunks(const DecayRuns a, const int first_run)
     static_assert(PIECES * N == C * (D / 8), "whole pieces");
     constexpr int ROWS = (OUT ? DOT ? 4 : 3 : 2) * NP * PLANE;
     __shared__ __attribute__((aligned(16))) __bf16 tile[ROWS];
-    __shared__ __attribute__((aligned(16))) __bf16 weights[OUT ? (KEEP + 1) * PPLANE : 8];
+    // (a single wave keeps the weights to itself)
+    __shared__ __attribute__((aligned(16))) __bf16 weights[OUT && W > 1 ? (KEEP + 1) * PPLANE : 8];
     __shared__ float pw[C + 1];
     __shared__ int strange[2];
     const DecayRun r = a.run[first_run + blockIdx.z];
@@ -405,9 +406,10 @@ void k_chunks(const DecayRuns a, const int first_run)
         if (tid == 0) strange[(c + 1) & 1] = 0;
         const int skip = c == 0 ? pad + (reverse && seg == 0 ? 1 : 0) : 0;      // steps by which the state's decay is short
 
+        constexpr int TILES = CT * (CT + 1) / 2;
+        bf16x4 own[W == 1 ? TILES : 1][KEEP + 1];
         if constexpr (OUT) {
             // the weights, each wave its tiles
-            constexpr int TILES = CT * (CT + 1) / 2;
 #pragma unroll
             for (int turn = 0; turn < (TILES + W - 1) / W; turn++) {
                 const int n = W == 1 ? turn : wave + turn * W;
@@ -425,8 +427,10 @@ void k_chunks(const DecayRuns a, const int first_run)
                 bf16x4 u[KEEP + 1];
                 split<KEEP + 1>(acc, u);
 #pragma unroll
-                for (int p = 0; p <= KEEP; p++)
-                    *(bf16x4*)(weights + p * PPLANE + (it * 16 + li) * PROW + jt * 16 + 4 * g) = u[p];
+                for (int p = 0; p <= KEEP; p++) {
+                    if constexpr (W == 1) own[turn][p] = u[p];
+                    else *(bf16x4*)(weights + p * PPLANE + (it * 16 + li) * PROW + jt * 16 + 4 * g) = u[p];
+                }
                 if constexpr (DOT) {
                     const f32x4 d = products(tz, tq, jt, it);
 #pragma unroll
@@ -545,15 +549,20 @@ void k_chunks(const DecayRuns a, const int first_run)
                 }
             }
         }
-        if constexpr (OUT) __syncthreads();                   // the weights are there
+        if constexpr (OUT && W > 1) __syncthreads();          // the weights are there
         if (OUT && works) {
             // P z, 32 earlier steps at a time
             const auto add_block = [&](int it, int k, auto careful) {
                 bf16x8 wp[KEEP + 1], zb[NP];
 #pragma unroll
                 for (int p = 0; p <= KEEP; p++) {
-                    const __bf16* at = weights + p * PPLANE + (it * 16 + li) * PROW + k * 32 + 4 * g;
-                    wp[p] = join(*(const bf16x4*)at, 2 * k + 1 <= it ? *(const bf16x4*)(at + 16) : bf16x4{});
+                    if constexpr (W == 1) {
+                        const int n = it * (it + 1) / 2 + 2 * k;
+                        wp[p] = join(own[n][p], 2 * k + 1 <= it ? own[n + 1][p] : bf16x4{});
+                    } else {
+                        const __bf16* at = weights + p * PPLANE + (it * 16 + li) * PROW + k * 32 + 4 * g;
+                        wp[p] = join(*(const bf16x4*)at, 2 * k + 1 <= it ? *(const bf16x4*)(at + 16) : bf16x4{});
+                    }
                 }
 #pragma unroll
                 for (int n = 0; n < NP; n++) {
