@@ -47,7 +47,7 @@ constexpr int decay_width(int e, int f)
     return w <= 16 ? 16 : w <= 32 ? 32 : w <= 64 ? 64 : 128;
 }
 
-// `n` runs starting at run[first]; slope: the run carries dS/dlog_decay; states_only: nothing but `carry` is written
-int decay_launch_f32(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream);
-int decay_launch_bf16(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream);
-int decay_launch_f16(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream);
+// `n` runs, the first `slopes` of them (none or one) with dS/dlog_decay; states_only: nothing but `carry` is written
+int decay_launch_f32(const DecayRuns& a, int n, int slopes, bool states_only, hipStream_t stream);
+int decay_launch_bf16(const DecayRuns& a, int n, int slopes, bool states_only, hipStream_t stream);
+int decay_launch_f16(const DecayRuns& a, int n, int slopes, bool states_only, hipStream_t stream);

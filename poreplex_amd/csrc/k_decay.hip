@@ -66,30 +66,25 @@ __global__ __launch_bounds__(256) void k_decay_sum(const double* partial, int64_
     if (threadIdx.x == 0) out[blockIdx.x] = (float)red[0];
 }
 
-int launch(const DecayRuns& a, int dtype, int first, int n, bool slope, bool states_only, hipStream_t stream)
+int launch(const DecayRuns& a, int dtype, int n, int slopes, bool states_only, hipStream_t stream)
 {
     switch (dtype) {
-    case PXG_DT_F32: return decay_launch_f32(a, first, n, slope, states_only, stream);
-    case PXG_DT_BF16: return decay_launch_bf16(a, first, n, slope, states_only, stream);
-    default: return decay_launch_f16(a, first, n, slope, states_only, stream);
+    case PXG_DT_F32: return decay_launch_f32(a, n, slopes, states_only, stream);
+    case PXG_DT_BF16: return decay_launch_bf16(a, n, slopes, states_only, stream);
+    default: return decay_launch_f16(a, n, slopes, states_only, stream);
     }
 }
 
-// The first `slope_runs` of the `n` runs carry slopes.
-int launch_runs(const DecayRuns& a, int dtype, int n, int slope_runs, hipStream_t stream)
+int launch_runs(const DecayRuns& a, int dtype, int n, int slopes, hipStream_t stream)
 {
-    int rc = PXG_OK;
     if (a.segments > 1) {
-        if (slope_runs) rc = launch(a, dtype, 0, slope_runs, true, true, stream);
-        if (rc == PXG_OK && n > slope_runs) rc = launch(a, dtype, slope_runs, n - slope_runs, false, true, stream);
+        const int rc = launch(a, dtype, n, slopes, true, stream);
         if (rc != PXG_OK) return rc;
         const dim3 grid(a.batch * a.heads, (a.run[0].E * a.run[0].F + 255) / 256, n);
-        k_decay_join<<<grid, 256, 0, stream>>>(a, decay_chunk(dtype, decay_width(a.run[0].E, a.run[0].F)), slope_runs);
+        k_decay_join<<<grid, 256, 0, stream>>>(a, decay_chunk(dtype, decay_width(a.run[0].E, a.run[0].F)), slopes);
         if (hipGetLastError() != hipSuccess) return PXG_E_HIP;
     }
-    if (slope_runs) rc = launch(a, dtype, 0, slope_runs, true, false, stream);
-    if (rc == PXG_OK && n > slope_runs) rc = launch(a, dtype, slope_runs, n - slope_runs, false, false, stream);
-    return rc;
+    return launch(a, dtype, n, slopes, false, stream);
 }
 
 // One step.  The state is read once and written once, 8 dk dv bytes for 5 dk dv operations: bandwidth is all there is.  P threads

@@ -200,12 +200,22 @@ constexpr int waves_wanted(int planes, int width, bool slope, bool states_only)
 {
     if (states_only) return 3;
     if (slope || (planes == 3 && (width == 16 || width == 128))) return 2;
-    return planes == 2 && width == 128 ? 4 : 3;
+    return planes < 3 && width >= 64 ? 4 : 3;
 }
 
+// Shared memory of one workgroup, as separate arrays: what is written to one does not hold up what is read from another.
+#define DECAY_SHARED(T, D, SLOPE, STATES_ONLY)                                                                                          \
+    constexpr int SETS = STATES_ONLY ? 2 : SLOPE ? 4 : 3, CHUNK = decay_chunk(Type<T>::code, D);                                      \
+    constexpr int WEIGHT_PLANES = STATES_ONLY || D == 16 ? 0 : Type<T>::planes == 3 ? 3 : 2;                                          \
+    __shared__ __attribute__((aligned(16))) __bf16 tile[SETS * Type<T>::planes * CHUNK * Shape<D>::row];                              \
+    __shared__ __attribute__((aligned(16))) __bf16 weights[WEIGHT_PLANES ? WEIGHT_PLANES * CHUNK * (CHUNK + 8) : 8];                  \
+    __shared__ float pw[CHUNK + 1];                                                                                                   \
+    __shared__ double sums[Shape<D>::waves];                                                                                          \
+    __shared__ int strange[2]
+
 template <typename T, int D, bool SLOPE, bool STATES_ONLY, bool WIDE>
-__global__ __launch_bounds__(Shape<D>::threads, waves_wanted(Type<T>::planes, D, SLOPE, STATES_ONLY))
-void k_chunks(const DecayRuns a, const int first_run)
+__device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& r, __bf16* const tile, __bf16* const weights,
+                                            float* const pw, double* const sums, int* const strange)
 {
     using Sh = Shape<D>;
     constexpr int NP = Type<T>::planes, C = decay_chunk(Type<T>::code, D), CT = C / 16, ET = Sh::et, KB = Sh::kb;
@@ -215,13 +225,6 @@ void k_chunks(const DecayRuns a, const int first_run)
     constexpr int SLOPE_PLANES = 3;
     constexpr bool OUT = !STATES_ONLY, DOT = SLOPE && OUT;
     static_assert(PIECES * N == C * (D / 8), "whole pieces");
-    constexpr int ROWS = (OUT ? DOT ? 4 : 3 : 2) * NP * PLANE;
-    __shared__ __attribute__((aligned(16))) __bf16 tile[ROWS];
-    // (a single wave keeps the weights to itself)
-    __shared__ __attribute__((aligned(16))) __bf16 weights[OUT && W > 1 ? (KEEP + 1) * PPLANE : 8];
-    __shared__ float pw[C + 1];
-    __shared__ int strange[2];
-    const DecayRun r = a.run[first_run + blockIdx.z];
     const int bh = xcd_order(blockIdx.x, gridDim.x), b = bh / a.heads, h = bh % a.heads, seg = blockIdx.y;
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, g = lane / 16, li = lane % 16, f0 = wave * 16;
     const int E = r.E, F = r.F;
@@ -682,7 +685,6 @@ void k_chunks(const DecayRuns a, const int first_run)
         total += (double)part;
 #pragma unroll
         for (int m = 32; m; m >>= 1) total += __shfl_xor(total, m);
-        __shared__ double sums[W];
         if (lane == 0) sums[wave] = total;
         __syncthreads();
         if (tid == 0) {
@@ -693,35 +695,57 @@ void k_chunks(const DecayRuns a, const int first_run)
     }
 }
 
-template <typename T, int D, bool WIDE>
-int launch_width(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream)
+template <typename T, int D, bool SLOPE, bool STATES_ONLY, bool WIDE>
+__global__ __launch_bounds__(Shape<D>::threads, waves_wanted(Type<T>::planes, D, SLOPE, STATES_ONLY))
+void k_chunks(const DecayRuns a, const int first_run)
 {
-    const dim3 grid(a.batch * a.heads, states_only ? a.segments - 1 : a.segments, n), block(Shape<D>::threads);
-    if (states_only) {
-        if (slope) k_chunks<T, D, true, true, WIDE><<<grid, block, 0, stream>>>(a, first);
-        else k_chunks<T, D, false, true, WIDE><<<grid, block, 0, stream>>>(a, first);
+    DECAY_SHARED(T, D, SLOPE, STATES_ONLY);
+    const DecayRun r = a.run[first_run + blockIdx.z];
+    walk_chunks<T, D, SLOPE, STATES_ONLY, WIDE>(a, r, tile, weights, pw, sums, strange);
+}
+
+// run 0 with slopes beside the others
+template <typename T, int D, bool STATES_ONLY, bool WIDE>
+__global__ __launch_bounds__(Shape<D>::threads, waves_wanted(Type<T>::planes, D, true, STATES_ONLY))
+void k_mixed_chunks(const DecayRuns a)
+{
+    DECAY_SHARED(T, D, true, STATES_ONLY);
+    const DecayRun r = a.run[blockIdx.z];
+    if (blockIdx.z == 0) walk_chunks<T, D, true, STATES_ONLY, WIDE>(a, r, tile, weights, pw, sums, strange);
+    else walk_chunks<T, D, false, STATES_ONLY, WIDE>(a, r, tile, weights, pw, sums, strange);
+}
+
+// The first `slopes` of the `n` runs (none or one) carry slopes.
+template <typename T, int D, bool STATES_ONLY, bool WIDE> int launch_width(const DecayRuns& a, int n, int slopes, hipStream_t stream)
+{
+    const dim3 block(Shape<D>::threads);
+    const auto grid = [&](int runs) { return dim3(a.batch * a.heads, STATES_ONLY ? a.segments - 1 : a.segments, runs); };
+    // side by side where the others do not lose waves to the registers that slopes take
+    if (slopes && n > slopes && !(Type<T>::planes == 2 && D == 128)) {
+        k_mixed_chunks<T, D, STATES_ONLY, WIDE><<<grid(n), block, 0, stream>>>(a);
     } else {
-        if (slope) k_chunks<T, D, true, false, WIDE><<<grid, block, 0, stream>>>(a, first);
-        else k_chunks<T, D, false, false, WIDE><<<grid, block, 0, stream>>>(a, first);
+        if (slopes) k_chunks<T, D, true, STATES_ONLY, WIDE><<<grid(slopes), block, 0, stream>>>(a, 0);
+        if (hipPeekAtLastError() == hipSuccess && n > slopes)
+            k_chunks<T, D, false, STATES_ONLY, WIDE><<<grid(n - slopes), block, 0, stream>>>(a, slopes);
     }
     return hipGetLastError() == hipSuccess ? PXG_OK : PXG_E_HIP;
 }
 
-template <typename T, int D> int launch_rows(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream)
+template <typename T, int D> int launch_rows(const DecayRuns& a, int n, int slopes, bool states_only, hipStream_t stream)
 {
     bool wide = true;
-    for (int i = first; i < first + n; i++) wide &= a.run[i].wide != 0;
-    return wide ? launch_width<T, D, true>(a, first, n, slope, states_only, stream)
-                : launch_width<T, D, false>(a, first, n, slope, states_only, stream);
+    for (int i = 0; i < n; i++) wide &= a.run[i].wide != 0;
+    if (states_only) return wide ? launch_width<T, D, true, true>(a, n, slopes, stream) : launch_width<T, D, true, false>(a, n, slopes, stream);
+    return wide ? launch_width<T, D, false, true>(a, n, slopes, stream) : launch_width<T, D, false, false>(a, n, slopes, stream);
 }
 
-template <typename T> int launch(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream)
+template <typename T> int launch(const DecayRuns& a, int n, int slopes, bool states_only, hipStream_t stream)
 {
-    switch (decay_width(a.run[first].E, a.run[first].F)) {
-    case 16: return launch_rows<T, 16>(a, first, n, slope, states_only, stream);
-    case 32: return launch_rows<T, 32>(a, first, n, slope, states_only, stream);
-    case 64: return launch_rows<T, 64>(a, first, n, slope, states_only, stream);
-    default: return launch_rows<T, 128>(a, first, n, slope, states_only, stream);
+    switch (decay_width(a.run[0].E, a.run[0].F)) {
+    case 16: return launch_rows<T, 16>(a, n, slopes, states_only, stream);
+    case 32: return launch_rows<T, 32>(a, n, slopes, states_only, stream);
+    case 64: return launch_rows<T, 64>(a, n, slopes, states_only, stream);
+    default: return launch_rows<T, 128>(a, n, slopes, states_only, stream);
     }
 }
 

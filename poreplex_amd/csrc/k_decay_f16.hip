@@ -2,7 +2,7 @@
 // side by side.
 #include "k_decay_chunk.h"
 
-int decay_launch_f16(const DecayRuns& a, int first, int n, bool slope, bool states_only, hipStream_t stream)
+int decay_launch_f16(const DecayRuns& a, int n, int slopes, bool states_only, hipStream_t stream)
 {
-    return decay::launch<pxg_f16>(a, first, n, slope, states_only, stream);
+    return decay::launch<pxg_f16>(a, n, slopes, states_only, stream);
 }
