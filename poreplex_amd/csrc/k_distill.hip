@@ -170,11 +170,10 @@ template <int G, typename T, typename F> __device__ __forceinline__ void each_un
 // of equal values, rows that only ascend) take their bound by bisection instead, reading the row again and again.
 //   2 047 x 50 001 bf16, k = 64: reading the row a second time for the sum, from whatever cache has it, took 101 us, keeping it in
 //   registers (which leaves room for few workgroups) 222, collecting elements instead of units' numbers 88.
-constexpr int CAND = 1024;
-
 template <int G> struct alignas(16) TopShared {
     static constexpr int parts = G < 256 ? G : 256, notes = G == 64 ? 256 : 2048;       // G = 64: up to 256 units
-    unsigned long long cand[CAND];              // (order, ~class): no two are equal
+    static constexpr int room = G == 64 ? 256 : 1024;
+    unsigned long long cand[room];              // (order, ~class): no two are equal
     uint32_t most[parts];
     double redd[G / 64];
     float redf[G / 64];
@@ -189,7 +188,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G)
 void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, int k, float temperature, T* values, int32_t* indices,
            float* rest)
 {
-    constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n, PARTS = TopShared<G>::parts, EACH = G / PARTS;
+    constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n, PARTS = TopShared<G>::parts, EACH = G / PARTS, CAND = TopShared<G>::room;
     __shared__ TopShared<G> shared[GROUPS];
     const int64_t row = (int64_t)blockIdx.x * GROUPS + (G == 64 ? threadIdx.x / 64 : 0);
     if (row >= rows) return;                    // a whole wave, or nobody

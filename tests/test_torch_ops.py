@@ -655,9 +655,7 @@ def dry(monkeypatch):
 
     def launched(*a):
         raise AssertionError('launched')
-    monkeypatch.setattr(ops, '_call', launched)
-    monkeypatch.setattr(ops, '_lib', launched)
-    monkeypatch.setattr(ops, '_differentiable', launched)
+    monkeypatch.setattr(ops, '_ext', launched)
 
 
 def test_cpu_tensors_are_refused():
