@@ -40,8 +40,8 @@ class ScalerNet(torch.nn.Module):
         w = load_model_arrays(bundle)
         self.l1 = keras_lstm(w['lstm1_kernel'], w['lstm1_recurrent'], w['lstm1_bias'])
         self.l2 = keras_lstm(w['lstm2_kernel'], w['lstm2_recurrent'], w['lstm2_bias'])
-        self.dk = torch.from_numpy(np.ascontiguousarray(w['dense_kernel']))
-        self.db = torch.from_numpy(np.ascontiguousarray(w['dense_bias']))
+        self.register_buffer('dk', torch.from_numpy(np.ascontiguousarray(w['dense_kernel'])), persistent=False)
+        self.register_buffer('db', torch.from_numpy(np.ascontiguousarray(w['dense_bias'])), persistent=False)
 
     def forward(self, x):
         h, _ = self.l1(x.unsqueeze(-1))
@@ -58,8 +58,8 @@ class DemuxNet(torch.nn.Module):
         self.fwd = keras_lstm(w['fwd_kernel'], w['fwd_recurrent'], w['fwd_bias'])
         self.bwd = keras_lstm(w['bwd_kernel'], w['bwd_recurrent'], w['bwd_bias'])
         self.top = keras_lstm(w['top_kernel'], w['top_recurrent'], w['top_bias'])
-        self.dk = torch.from_numpy(np.ascontiguousarray(w['dense_kernel']))
-        self.db = torch.from_numpy(np.ascontiguousarray(w['dense_bias']))
+        self.register_buffer('dk', torch.from_numpy(np.ascontiguousarray(w['dense_kernel'])), persistent=False)
+        self.register_buffer('db', torch.from_numpy(np.ascontiguousarray(w['dense_bias'])), persistent=False)
 
     def forward(self, x):
         x = x.unsqueeze(-1)

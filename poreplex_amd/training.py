@@ -19,6 +19,14 @@ models are Keras graphs trained under tf.distribute.MirroredStrategy; here:
     i, f, c, o), so a trained model drops into ``pxg_create`` unchanged; the demux bundle
     carries a calibration table (phred -> minimal score) fitted on held-out predictions.
 
+A network can also be taught by another one instead of by labels: ``distillation_targets`` asks the
+teacher (the shipped classifier, ``torch_models.DemuxNet``, or any module that returns logits) once
+for its largest answers to every sample, and ``Trainer`` takes them as its targets with
+``torch_ops.distillation_loss`` as its loss.  ``DemuxClassifier(top='decay')`` is a classifier whose
+top layer is ``DecayRecurrence`` -- linear attention with a decay per head on the HIP kernels of
+``torch_ops`` -- in the place of an LSTM; the signal path's kernels hold LSTM weights only, so it is
+not exported.
+
 No real training data exists in this repository: ``synthetic_demux_dataset`` /
 ``synthetic_scaler_dataset`` draw from the same generator as the bench reads.
 """
@@ -29,7 +37,8 @@ import numpy as np
 import torch
 from torch import nn
 
-__all__ = ['DemuxClassifier', 'ScalerRegressor', 'Trainer', 'weighted_cross_entropy',
+__all__ = ['DemuxClassifier', 'ScalerRegressor', 'DecayRecurrence', 'Trainer', 'weighted_cross_entropy',
+           'distillation_targets',
            'weighted_accuracy', 'fit_calibration', 'export_demux_bundle', 'export_scaler_bundle',
            'synthetic_demux_dataset', 'synthetic_scaler_dataset']
 
@@ -51,14 +60,55 @@ class _KerasLSTM(nn.LSTM):
                 self.bias_ih_l0.detach().cpu().numpy().copy())
 
 
-class DemuxClassifier(nn.Module):
-    """[B, 300] normalised adapter windows -> log-probabilities [B, n_classes]."""
+class DecayRecurrence(nn.Module):
+    """A recurrent layer whose time axis is not serial: `heads` states of [units / heads] x [units / heads] that
+    decay at a learned rate (torch_ops.decay_attention; GPU only).  Called like an LSTM layer on [B, T, inputs] ->
+    ([B, T, units], state); `step` takes one sample of many streams and updates their states in place."""
 
-    def __init__(self, n_classes=5, noise=0.05, drop1=0.2, drop2=0.3):
+    def __init__(self, inputs, units, heads=4):
         super().__init__()
+        if units % heads:
+            raise ValueError('{} units over {} heads'.format(units, heads))
+        self.heads, self.width = heads, units // heads
+        self.qkv = nn.Linear(inputs, 3 * units)
+        self.out = nn.Linear(units, units)
+        # half of a head's memory is gone after 2 ^ (2 .. 7) steps or so; the decay stays below 1 whatever is learned
+        spans = torch.exp2(torch.linspace(3.0, 8.0, heads))
+        self.rate = nn.Parameter(torch.log(-torch.log1p(-1.0 / spans)))
+
+    def _heads(self, x):
+        q, k, v = self.qkv(x).unflatten(-1, (3, self.heads, self.width)).unbind(-3)
+        return q * self.width ** -0.5, k, v
+
+    def new_state(self, batch, device=None):
+        return torch.zeros(batch, self.heads, self.width, self.width, device=self.rate.device if device is None else device)
+
+    def forward(self, x, lengths=None, state=None):
+        from . import torch_ops
+        q, k, v = self._heads(x)
+        o, state = torch_ops.decay_attention(q, k, v, -torch.exp(self.rate.float()), lengths, state, return_state=True)
+        return self.out(o.flatten(-2)), state
+
+    def step(self, x, state, active=None):
+        """[B, inputs] -> [B, units]; `state` (new_state, or what forward returned) is updated in place."""
+        from . import torch_ops
+        with torch.no_grad():
+            q, k, v = self._heads(x)
+            o = torch_ops.decay_attention_step(q, k, v, -torch.exp(self.rate.float()), state, active)
+            return self.out(o.flatten(-2))
+
+
+class DemuxClassifier(nn.Module):
+    """[B, 300] normalised adapter windows -> log-probabilities [B, n_classes].  `top`: 'lstm' as in the shipped
+    model, or 'decay' (DecayRecurrence)."""
+
+    def __init__(self, n_classes=5, noise=0.05, drop1=0.2, drop2=0.3, top='lstm'):
+        super().__init__()
+        if top not in ('lstm', 'decay'):
+            raise ValueError("top is {!r}: 'lstm' or 'decay'".format(top))
         self.noise = noise
         self.fwd, self.bwd = _KerasLSTM(1, 48), _KerasLSTM(1, 48)
-        self.top = _KerasLSTM(96, 64)
+        self.top = _KerasLSTM(96, 64) if top == 'lstm' else DecayRecurrence(96, 64)
         self.drop1, self.drop2 = nn.Dropout(drop1), nn.Dropout(drop2)
         self.dense = nn.Linear(64, n_classes)
 
@@ -69,8 +119,12 @@ class DemuxClassifier(nn.Module):
         hf, _ = self.fwd(x)
         hb, _ = self.bwd(torch.flip(x, dims=[1]))
         h = self.drop1(torch.cat([hf, torch.flip(hb, dims=[1])], dim=-1))
-        _, (hn, _) = self.top(h)
-        return torch.log_softmax(self.dense(self.drop2(hn[0])), dim=-1)
+        if isinstance(self.top, DecayRecurrence):
+            last = self.top(h)[0][:, -1]
+        else:
+            _, (hn, _) = self.top(h)
+            last = hn[0]
+        return torch.log_softmax(self.dense(self.drop2(last)), dim=-1)
 
 
 class ScalerRegressor(nn.Module):
@@ -116,6 +170,19 @@ def weighted_cross_entropy(logp, labels, cost, class_weight=None):
 def weighted_accuracy(logp, labels, cost):
     w = _sample_weights(logp, labels, cost)
     return float((w * (logp.argmax(dim=1) == labels)).sum() / w.sum())
+
+
+def distillation_targets(teacher, x, k=3, temperature=2.0, device='cuda', batch_size=4096):
+    """The teacher's `k` largest answers to every sample of x (torch_ops.TopLogits on the CPU): the targets of
+    ``Trainer(model, torch_ops.distillation_loss).fit(x, targets)``."""
+    from . import torch_ops
+    device, parts = torch.device(device), []
+    teacher = teacher.to(device).eval()
+    with torch.no_grad():
+        for a in range(0, len(x), batch_size):
+            logits = teacher(x[a:a + batch_size].to(device))
+            parts.append(torch_ops.top_logits(logits, min(k, logits.shape[1]), temperature).to('cpu'))
+    return torch_ops.TopLogits.cat(parts)
 
 
 # ---- trainer -----------------------------------------------------------------------------
@@ -230,6 +297,8 @@ def fit_calibration(scores, correct, n_rows=29):
 
 
 def export_demux_bundle(model, path, calibration):
+    if isinstance(model.top, DecayRecurrence):
+        raise ValueError('a classifier with a decay recurrence cannot be exported: the signal path\'s kernels hold LSTM weights')
     arrays = {}
     for name, layer in (('fwd', model.fwd), ('bwd', model.bwd), ('top', model.top)):
         k, r, b = layer.keras_arrays()
