@@ -270,6 +270,7 @@ extern "C" int pxg_decay_forward(const pxg_decay* a, void* stream)
     r.out = a->out, r.E = a->dk, r.F = a->dv;
     r.carry = (float*)a->workspace;
     finish_run(r, a->dtype);
+    (void)hipGetLastError();                     // what an earlier call left is not this call's
     return launch_runs(s, a->dtype, 1, 0, (hipStream_t)stream);
 }
 
@@ -281,6 +282,7 @@ extern "C" int pxg_decay_backward(const pxg_decay* a, void* stream)
     const int64_t bytes = pxg_decay_workspace_bytes(a, 1);
     if (a->workspace_bytes < bytes || (bytes > 0 && !a->workspace)) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
+    (void)hipGetLastError();                     // what an earlier call left is not this call's
     const Cut c = cut_of(a, true);
     DecayRuns s = runs_of(a, c);
     double* const partial = (double*)a->workspace;
@@ -315,6 +317,7 @@ extern "C" int pxg_decay_step(const pxg_decay* a, void* stream)
     if (a->batch == 0) return PXG_OK;
     if (!a->out || !a->final_state) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
+    (void)hipGetLastError();                     // what an earlier call left is not this call's
     switch (a->dtype) {
     case PXG_DT_F32: launch_step<float>(*a, st); break;
     case PXG_DT_BF16: launch_step<pxg_bf16>(*a, st); break;

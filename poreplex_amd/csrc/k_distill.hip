@@ -725,6 +725,7 @@ extern "C" int pxg_top_logits(int32_t dtype, int64_t rows, int64_t classes, cons
     if (rows == 0) return PXG_OK;
     if (!logits || !values || !indices || !rest) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
+    (void)hipGetLastError();                     // what an earlier call left is not this call's
     switch (dtype) {
     case PXG_DT_F32: launch_top<float>(rows, classes, logits, row_stride, k, temperature, values, indices, rest, st); break;
     case PXG_DT_BF16: launch_top<pxg_bf16>(rows, classes, logits, row_stride, k, temperature, values, indices, rest, st); break;
@@ -737,6 +738,7 @@ extern "C" int pxg_distill_forward(const pxg_distill* a, void* stream)
 {
     if (bad_call(a) || (a->rows > 0 && !a->row_loss)) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
+    (void)hipGetLastError();                     // what an earlier call left is not this call's
     if (a->rows) {
         switch (a->dtype) {
         case PXG_DT_F32: launch_forward<float>(*a, st); break;
@@ -758,6 +760,7 @@ extern "C" int pxg_distill_backward(const pxg_distill* a, void* stream)
     if (a->rows == 0) return PXG_OK;
     if (!a->grad_loss || !a->grad_logits) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
+    (void)hipGetLastError();                     // what an earlier call left is not this call's
     switch (a->dtype) {
     case PXG_DT_F32: launch_backward<float>(*a, st); break;
     case PXG_DT_BF16: launch_backward<pxg_bf16>(*a, st); break;

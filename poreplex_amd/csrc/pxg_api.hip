@@ -767,8 +767,12 @@ extern "C" int pxg_host_register(pxg_ctx* ctx, void* ptr, size_t bytes)
 {
     if (!ctx || !ptr || !bytes) return PXG_E_INVALID;
     PXG_HIP(ctx, hipSetDevice(ctx->device));
-    PXG_HIP(ctx, hipHostRegister(ptr, bytes, hipHostRegisterDefault));
-    return PXG_OK;
+    const hipError_t e = hipHostRegister(ptr, bytes, hipHostRegisterDefault);
+    if (e == hipSuccess) return PXG_OK;
+    (void)hipGetLastError();                     // or the next call on any stream would report it as its own
+    pxg_set_err(ctx, std::string("hipHostRegister: ") + hipGetErrorString(e));
+    // some machines lock no memory that already exists: the copies then go through the context's own page-locked chunks
+    return e == hipErrorInvalidValue || e == hipErrorNotSupported ? PXG_E_UNSUPPORTED : PXG_E_HIP;
 }
 
 extern "C" int pxg_host_unregister(pxg_ctx* ctx, void* ptr)
@@ -781,8 +785,11 @@ extern "C" int pxg_host_unregister(pxg_ctx* ctx, void* ptr)
         (void)hipGetLastError();
         return PXG_E_HIP;
     }
-    PXG_HIP(ctx, hipHostUnregister(ptr));
-    return PXG_OK;
+    const hipError_t e = hipHostUnregister(ptr);
+    if (e == hipSuccess) return PXG_OK;
+    (void)hipGetLastError();
+    pxg_set_err(ctx, std::string("hipHostUnregister: ") + hipGetErrorString(e));
+    return PXG_E_HIP;
 }
 
 #define PXG_POLYA_BESIDE_MAX 20000

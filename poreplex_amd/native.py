@@ -955,9 +955,14 @@ class NativeContext:
         self._staged = None
 
     def pin(self, array):
-        """Page-lock a NumPy array so stage() copies are DMA transfers; returns it."""
-        self._check(self.lib.pxg_host_register(self.handle, _ptr(array), array.nbytes),
-                    'pxg_host_register')
+        """Page-lock a NumPy array so stage() copies are DMA transfers; returns it.  Where the machine locks no
+        memory that already exists the array stays pageable: slower copies, the same results."""
+        rc = self.lib.pxg_host_register(self.handle, _ptr(array), array.nbytes)
+        if rc == PXG_E_UNSUPPORTED:
+            self._unlocked = getattr(self, '_unlocked', set())
+            self._unlocked.add(_ptr(array).value)
+            return array
+        self._check(rc, 'pxg_host_register')
         self._pinned = getattr(self, '_pinned', {})
         self._pinned[_ptr(array).value] = array       # (kept alive until it is released)
         return array
@@ -965,6 +970,10 @@ class NativeContext:
     def unpin(self, array):
         """Release a page lock.  Works after close() too (page locks are process-global): a staging arena
         that outlives its context is released, not left registered on memory about to be unmapped."""
+        unlocked = getattr(self, '_unlocked', ())
+        if _ptr(array).value in unlocked:
+            unlocked.discard(_ptr(array).value)
+            return
         getattr(self, '_pinned', {}).pop(_ptr(array).value, None)
         rc = self.lib.pxg_host_unregister(self.handle if getattr(self, 'handle', None) else None, _ptr(array))
         if rc != 0:
