@@ -658,13 +658,15 @@ int pxg_h5_basecall_many(int64_t n, const pxg_h5* const* files, const int64_t* i
  * Every pointer below is device memory of the CURRENT HIP device; `stream` is a hipStream_t of that device (NULL: its
  * default stream).  The calls only launch kernels: no allocation, no synchronisation, no memset, so they may be captured
  * into a graph.  Work that needs scratch memory takes it from the caller (`workspace`, at least as many bytes as the
- * *_workspace_bytes function says, not shared by calls that may run at once); its contents before and after mean nothing.
+ * *_workspace_bytes function says, at an address that is a multiple of 8, not shared by calls that may run at once); its
+ * contents before and after mean nothing.  No output may overlap an input, other than the state of pxg_decay_step.
  * Values are checked where the host can see them (shapes, types, pointers): PXG_E_INVALID; what lies in device memory
  * (lengths, class indices) is bounded by the kernels themselves.  No context is needed; calls from several threads are
  * independent of each other. */
 enum pxg_dtype { PXG_DT_F32 = 0, PXG_DT_BF16 = 1, PXG_DT_F16 = 2 };
 
 #define PXG_DECAY_MAX_WIDTH 128    /* largest dk and dv */
+#define PXG_DECAY_MAX_PAIRS 8388607 /* largest batch * heads: workgroups of 512 threads in a grid of less than 2^32 threads */
 #define PXG_TOP_MAX_K       128    /* largest k of the top logits */
 
 /* A [batch][step][head][width] tensor: width is contiguous, the other strides are free (in elements, 0 for a broadcast). */
@@ -676,7 +678,8 @@ typedef struct {
 /* Linear attention with one decay a_h = exp(log_decay[h]) per head, a recurrence over the steps of each sequence:
  *     S_t = a_h S_(t-1) + k_t v_t^T        o_t = q_t S_t        S_(-1) = initial_state (0 where NULL)
  * Steps at or behind lengths[b] are neither read nor part of the state; their rows of `out` and of the gradients are 0.
- * A length below 0 counts as 0, one above `steps` as `steps`. */
+ * A length below 0 counts as 0, one above `steps` as `steps`.  A log_decay above 0 grows; the results are numbers while
+ * exp(log_decay * steps) is one. */
 typedef struct {
     uint32_t struct_bytes;            /* sizeof(pxg_decay) */
     int32_t dtype;                    /* pxg_dtype of q, k, v, out, grad_out and the gradients of q, k, v */
@@ -690,7 +693,7 @@ typedef struct {
     void* out;                        /* [batch][steps][heads][dv] */
     float* final_state;               /* [batch][heads][dk][dv] or NULL */
     /* pxg_decay_backward only */
-    pxg_sequence grad_out;            /* data may be NULL: all zero */
+    pxg_sequence grad_out;            /* like out */
     const float* grad_final_state;    /* or NULL */
     void *grad_q, *grad_k, *grad_v;   /* contiguous like q, k, v */
     float* grad_log_decay;            /* [heads] or NULL: not wanted */

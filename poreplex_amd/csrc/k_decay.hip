@@ -182,8 +182,8 @@ template <typename T> void launch_step(const pxg_decay& a, hipStream_t stream)
 bool bad_shape(const pxg_decay* a)
 {
     return !a || a->struct_bytes != sizeof(pxg_decay) || a->dtype < PXG_DT_F32 || a->dtype > PXG_DT_F16 || a->batch < 0 ||
-           a->steps < 0 || a->steps > INT32_MAX || a->heads < 1 || a->dk < 1 || a->dk > PXG_DECAY_MAX_WIDTH || a->dv < 1 ||
-           a->dv > PXG_DECAY_MAX_WIDTH || a->batch > INT32_MAX / a->heads;
+           a->steps < 0 || a->steps > INT32_MAX || a->heads < 1 || a->heads > PXG_DECAY_MAX_PAIRS || a->dk < 1 || a->dk > PXG_DECAY_MAX_WIDTH || a->dv < 1 ||
+           a->dv > PXG_DECAY_MAX_WIDTH || a->batch > PXG_DECAY_MAX_PAIRS / a->heads;
 }
 
 // a pointer may be missing only where nothing is read or written through it
@@ -262,7 +262,7 @@ extern "C" int pxg_decay_forward(const pxg_decay* a, void* stream)
     if (a->batch == 0) return PXG_OK;
     if (a->steps > 0 && !a->out) return PXG_E_INVALID;
     const int64_t bytes = pxg_decay_workspace_bytes(a, 0);
-    if (a->workspace_bytes < bytes || (bytes > 0 && !a->workspace)) return PXG_E_INVALID;
+    if (a->workspace_bytes < bytes || (bytes > 0 && (!a->workspace || (uintptr_t)a->workspace % 8))) return PXG_E_INVALID;
     DecayRuns s = runs_of(a, cut_of(a, false));
     DecayRun& r = s.run[0];
     r.x = a->q, r.y = a->k, r.z = a->v;
@@ -280,7 +280,7 @@ extern "C" int pxg_decay_backward(const pxg_decay* a, void* stream)
     const bool any = a->batch > 0 && a->steps > 0;
     if (any && (!a->grad_q || !a->grad_k || !a->grad_v || !a->grad_out.data)) return PXG_E_INVALID;
     const int64_t bytes = pxg_decay_workspace_bytes(a, 1);
-    if (a->workspace_bytes < bytes || (bytes > 0 && !a->workspace)) return PXG_E_INVALID;
+    if (a->workspace_bytes < bytes || (bytes > 0 && (!a->workspace || (uintptr_t)a->workspace % 8))) return PXG_E_INVALID;
     hipStream_t st = (hipStream_t)stream;
     (void)hipGetLastError();                     // what an earlier call left is not this call's
     const Cut c = cut_of(a, true);

@@ -28,6 +28,13 @@ template <int G> __device__ __forceinline__ void group_sync()
     }
 }
 
+// rows in the order of the workgroups, which lie in a grid of two axes where one would hold 2^32 threads or more
+template <int G> __device__ __forceinline__ int64_t row_of()
+{
+    const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+    return G == 64 ? block * 4 + threadIdx.x / 64 : block;
+}
+
 struct MaxOf { template <typename V> __device__ V operator()(V a, V b) const { return a > b ? a : b; } };
 struct SumOf { template <typename V> __device__ V operator()(V a, V b) const { return a + b; } };
 
@@ -176,6 +183,7 @@ template <int G> struct alignas(16) TopShared {
     unsigned long long cand[room];              // (order, ~class): no two are equal
     uint32_t most[parts];
     double redd[G / 64];
+    long long redi[G / 64];
     float redf[G / 64];
     int red[G / 64];
     uint32_t note[notes];
@@ -190,7 +198,7 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
 {
     constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n, PARTS = TopShared<G>::parts, EACH = G / PARTS, CAND = TopShared<G>::room;
     __shared__ TopShared<G> shared[GROUPS];
-    const int64_t row = (int64_t)blockIdx.x * GROUPS + (G == 64 ? threadIdx.x / 64 : 0);
+    const int64_t row = row_of<G>();
     if (row >= rows) return;                    // a whole wave, or nobody
     TopShared<G>& s = shared[G == 64 ? threadIdx.x / 64 : 0];
     const int t = threadIdx.x % G;
@@ -279,26 +287,25 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
     if (classes >= (int64_t)G * n) raise_bound();
     group_sync<G>();
     const int noted = s.noted;
-    if (noted <= TopShared<G>::notes)
+    bool listed = noted <= TopShared<G>::notes;
+    float most = -INFINITY;                     // of what is below the bound in the noted units
+    if (listed)
         for (int i = t; i < noted; i += G) {
             const int64_t unit = s.note[i];
             const Unit<T> u = load_unit(x, unit, classes);
-            float below[n], most = -INFINITY;
 #pragma unroll
             for (int e = 0; e < n; e++) {
                 const float v = pxg_to_f32(u.v[e]);
-                const bool is = v < bound;
-                below[e] = is ? v : -INFINITY;
-                most = fmaxf(most, below[e]);
-                if (!is && unit * n + e < classes) {
+                if (v < bound) {
+                    most = fmaxf(most, v);
+                } else if (unit * n + e < classes) {
                     const int at = atomicAdd(&s.count, 1);
                     if (at < CAND) s.cand[at] = (unsigned long long)order_of(v) << 32 | (uint32_t)~(uint32_t)(unit * n + e);
                 }
             }
-            sum.add(below, most, scale);
         }
     group_sync<G>();
-    int found = noted <= TopShared<G>::notes ? s.count : CAND + 1;
+    int found = listed ? s.count : CAND + 1;
     bool no_number = false;                     // among the rest (bisection only: otherwise it is a candidate)
     if (found > CAND) {
         // the largest key that k elements reach, bit by bit; then the smallest class below which enough of the ties lie
@@ -323,7 +330,7 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
             if (count([&](uint32_t o, uint32_t c) { return o == key && c < mid; }) >= need) high = mid;
             else low = mid;
         }
-        found = k;
+        found = k, listed = false, most = -INFINITY;
         if (t == 0) s.count = 0;
         group_sync<G>();
         sum = RunningSum<T>();
@@ -343,10 +350,25 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
         no_number = group_reduce<G>((int)strange, s.red, MaxOf());
         group_sync<G>();
     }
-    const float base = group_reduce<G>(sum.base, s.redf, MaxOf());
-    const double below = group_reduce<G>(sum.sum == 0.f ? 0.0 : (double)sum.sum * (double)exp_from<T>(sum.base, base, scale), s.redd, SumOf());
+    // What is noted comes in another order in every run: its sum is taken in whole multiples of 2^-44 of the largest term, which no
+    // order changes.
+    const auto whole_part = [](double part) { return (long long)rint(part * 0x1p44); };
+    const float base = group_reduce<G>(fmaxf(sum.base, most), s.redf, MaxOf());
+    double below = group_reduce<G>(sum.sum == 0.f ? 0.0 : (double)sum.sum * (double)exp_from<T>(sum.base, base, scale), s.redd, SumOf());
+    if (listed) {
+        long long parts = 0;
+        for (int i = t; i < noted; i += G) {
+            const Unit<T> u = load_unit(x, s.note[i], classes);
+#pragma unroll
+            for (int e = 0; e < n; e++) {
+                const float v = pxg_to_f32(u.v[e]);
+                if (v < bound) parts += whole_part(exp_from<T>(v, base, scale));
+            }
+        }
+        below += (double)group_reduce<G>(parts, s.redi, SumOf()) * 0x1p-44;
+    }
     // rank the candidates; the first k are the answer, the rest join the sum against the largest of them
-    double extra = 0.0;
+    long long extra = 0;
     const bool left = found > k;
     int rank[(CAND + G - 1) / G];
 #pragma unroll
@@ -375,14 +397,14 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
 #pragma unroll
             for (int a = 0; a < (CAND + G - 1) / G; a++)
                 if (t + a * G < found && rank[a] >= k)
-                    extra += exp(((double)value_of((uint32_t)(s.cand[t + a * G] >> 32)) - (double)top) / (double)temperature);
+                    extra += whole_part(exp(((double)value_of((uint32_t)(s.cand[t + a * G] >> 32)) - (double)top) / (double)temperature));
         }
-        extra = group_reduce<G>(extra, s.redd, SumOf());
+        extra = group_reduce<G>(extra, s.redi, SumOf());
     }
     if (t == 0) {
         double r;
         if (left && !__builtin_isfinite(top)) r = top;                     // -inf: so is all the rest
-        else if (left) r = (double)top / temperature + log(extra + (below > 0.0 ? below * exp(((double)base - top) / temperature) : 0.0));
+        else if (left) r = (double)top / temperature + log((double)extra * 0x1p-44 + (below > 0.0 ? below * exp(((double)base - top) / temperature) : 0.0));
         else if (no_number) r = NAN;
         else if (base == INFINITY) r = INFINITY;
         else r = below > 0.0 ? (double)base / temperature + log(below) : -INFINITY;
@@ -452,7 +474,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_forward(const pxg
 {
     constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n, PLACES = (PXG_TOP_MAX_K + G - 1) / G;
     __shared__ LossShared<G> shared[GROUPS];
-    const int64_t row = (int64_t)blockIdx.x * GROUPS + (G == 64 ? threadIdx.x / 64 : 0);
+    const int64_t row = row_of<G>();
     if (row >= a.rows) return;
     LossShared<G>& s = shared[G == 64 ? threadIdx.x / 64 : 0];
     const int t = threadIdx.x % G, k = a.k;
@@ -605,7 +627,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_backward(const px
 {
     constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n;
     __shared__ Marks<G> shared[GROUPS];
-    const int64_t row = (int64_t)blockIdx.x * GROUPS + (G == 64 ? threadIdx.x / 64 : 0);
+    const int64_t row = row_of<G>();
     if (row >= a.rows) return;
     Marks<G>& marks = shared[G == 64 ? threadIdx.x / 64 : 0];
     const int t = threadIdx.x % G, k = a.k;
@@ -668,7 +690,11 @@ int threads_of(int64_t rows, int64_t classes)
     return classes <= 1024 ? 64 : rows < 256 && classes > 16384 ? 1024 : 256;
 }
 
-unsigned blocks_of(int64_t rows, int threads) { return (unsigned)(threads == 64 ? (rows + 3) / 4 : rows); }
+dim3 blocks_of(int64_t rows, int threads)
+{
+    const int64_t n = threads == 64 ? (rows + 3) / 4 : rows, x = n < 1 << 21 ? n : 1 << 21;
+    return dim3((unsigned)x, (unsigned)((n + x - 1) / x));
+}
 
 template <typename T>
 void launch_top(int64_t rows, int64_t classes, const void* logits, int64_t row_stride, int k, float temperature, void* values,
@@ -676,7 +702,7 @@ void launch_top(int64_t rows, int64_t classes, const void* logits, int64_t row_s
 {
     int g = threads_of(rows, classes);
     if (k > 32 && g == 64) g = 256;                               // twice as many threads as are to be chosen
-    const unsigned blocks = blocks_of(rows, g);
+    const dim3 blocks = blocks_of(rows, g);
     switch (g) {
     case 64: k_top<64, T><<<blocks, 256, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest); break;
     case 256: k_top<256, T><<<blocks, 256, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest); break;
@@ -687,7 +713,7 @@ void launch_top(int64_t rows, int64_t classes, const void* logits, int64_t row_s
 template <typename T> void launch_forward(const pxg_distill& a, hipStream_t st)
 {
     const int g = threads_of(a.rows, a.classes);
-    const unsigned blocks = blocks_of(a.rows, g);
+    const dim3 blocks = blocks_of(a.rows, g);
     switch (g) {
     case 64: k_distill_forward<64, T><<<blocks, 256, 0, st>>>(a); break;
     case 256: k_distill_forward<256, T><<<blocks, 256, 0, st>>>(a); break;
@@ -698,7 +724,7 @@ template <typename T> void launch_forward(const pxg_distill& a, hipStream_t st)
 template <typename T> void launch_backward(const pxg_distill& a, hipStream_t st)
 {
     const int g = threads_of(a.rows, a.classes);
-    const unsigned blocks = blocks_of(a.rows, g);
+    const dim3 blocks = blocks_of(a.rows, g);
     switch (g) {
     case 64: k_distill_backward<64, T><<<blocks, 256, 0, st>>>(a); break;
     case 256: k_distill_backward<256, T><<<blocks, 256, 0, st>>>(a); break;

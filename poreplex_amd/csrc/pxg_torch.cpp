@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/utils/pybind.h>
+#include <unordered_set>
 #include "../../include/pxg.h"
 
 namespace py = pybind11;
@@ -71,18 +72,32 @@ template <typename V> V* data(const Tensor& t) { return t.defined() ? (V*)t.data
 Tensor empty(at::IntArrayRef shape, const Tensor& like, at::ScalarType type) { return at::empty(shape, like.options().dtype(type).requires_grad(false)); }
 
 // A leaf's gradient is accumulated on the stream where its oldest living graph was built.  Captured on another stream, the backward
-// pass would have to wait for that stream from inside the capture, which ends the process: refused here instead.
+// pass would have to wait for that stream from inside the capture, which ends the process: refused here instead, for every leaf
+// that the arguments come from.
 void refuse_captured_leaves(std::initializer_list<const Tensor*> tensors, const Tensor& any)
 {
     if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
     const auto now = c10::hip::getCurrentHIPStream(any.device().index());
+    std::vector<torch::autograd::Node*> todo;
+    std::unordered_set<torch::autograd::Node*> seen;
+    const auto visit = [&](torch::autograd::Node* node) {
+        if (node && seen.insert(node).second) todo.push_back(node);
+    };
+    std::vector<std::shared_ptr<torch::autograd::Node>> held;
     for (const Tensor* t : tensors) {
-        if (!t->defined() || !t->requires_grad() || t->grad_fn()) continue;
-        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        if (node && node->stream() && node->stream()->id() != now.id())
+        if (!t->defined() || !t->requires_grad()) continue;
+        held.push_back(t->grad_fn() ? t->grad_fn() : torch::autograd::impl::try_get_grad_accumulator(*t));
+        visit(held.back().get());
+    }
+    while (!todo.empty()) {
+        torch::autograd::Node* const node = todo.back();
+        todo.pop_back();
+        const bool leaf = node->num_outputs() == 0;           // it passes nothing on: it accumulates
+        if (leaf && node->stream() && node->stream()->id() != now.id())
             TORCH_CHECK(false, "capturing a differentiable call while a graph of the same leaf, built on another stream outside the "
                         "capture, is alive: free that graph first, or capture decay_attention_backward / "
                         "distillation_loss_and_gradient, which need no autograd graph");
+        for (const auto& edge : node->next_edges()) visit(edge.function.get());
     }
 }
 

@@ -26,6 +26,7 @@ PXG_MAX_CALIBRATION = 64
 UNSPLIT_E_GEOMETRY = -3
 UNSPLIT_E_WINDOW = -4
 PXG_DECAY_MAX_WIDTH = 128
+PXG_DECAY_MAX_PAIRS = 8388607
 PXG_TOP_MAX_K = 128
 
 STATUS_NAMES = (

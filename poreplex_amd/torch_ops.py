@@ -16,6 +16,7 @@ Arguments are checked here; csrc/pxg_torch.cpp makes the calls and is the autogr
 import ctypes as C
 import importlib.machinery
 import importlib.util
+import operator
 import os
 
 import torch
@@ -26,6 +27,7 @@ __all__ = ['TopLogits', 'decay_attention', 'decay_attention_backward', 'decay_at
            'distillation_loss_and_gradient', 'top_logits', 'MAX_WIDTH', 'MAX_K']
 
 MAX_WIDTH = _native.PXG_DECAY_MAX_WIDTH
+_MAX_PAIRS = _native.PXG_DECAY_MAX_PAIRS
 MAX_K = _native.PXG_TOP_MAX_K
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)                    # enum pxg_dtype
@@ -94,6 +96,8 @@ def _check_decay(q, k, v, log_decay, lengths, initial_state, steps_axis=True):
     batch, heads, dk, dv = q.shape[0], q.shape[-2], q.shape[-1], v.shape[-1]
     if not (1 <= dk <= MAX_WIDTH and 1 <= dv <= MAX_WIDTH and heads >= 1):
         raise ValueError('{} heads of widths {} and {}: at least one head, widths of 1 to {}'.format(heads, dk, dv, MAX_WIDTH))
+    if batch * heads > _MAX_PAIRS:
+        raise ValueError('{} sequences of {} heads: at most {} of both together'.format(batch, heads, _MAX_PAIRS))
     _f32('log_decay', log_decay, (heads,), device)
     if lengths is not None:
         _on_gpu('lengths', lengths, device)
@@ -111,8 +115,9 @@ def decay_attention(q, k, v, log_decay, lengths=None, initial_state=None, return
         S_t = exp(log_decay[h]) S_(t-1) + k_t v_t^T,    o_t = q_t S_t
 
     q, k [batch, steps, heads, dk] and v [batch, steps, heads, dv], float32, bfloat16 or float16, dk and dv of 1 to 128, any
-    strides (k and v that heads share are ``expand``-ed views); log_decay [heads] float32 (-inf: no memory).  lengths [batch]
-    (int32 or int64): the steps of each sequence; what lies behind them is not read, and its rows of the result are 0.
+    strides (k and v that heads share are ``expand``-ed views); log_decay [heads] float32 (-inf: no memory; one above 0
+    grows, and the result is a number while exp(log_decay * steps) is one).  lengths [batch] (int32 or int64): the steps of each
+    sequence, taken as 0 to steps; what lies behind them is not read, and its rows of the result are 0.
     initial_state [batch, heads, dk, dv] float32: S before the first step, 0 if None.
 
     Returns o [batch, steps, heads, dv] in v's type, or (o, S behind each sequence's last step, float32).  Differentiable in q,
@@ -170,7 +175,7 @@ class TopLogits:
         return TopLogits(self.values[rows], self.indices[rows], None if self.rest is None else self.rest[rows], self.temperature)
 
     def to(self, *args, **kwargs):
-        device = torch.empty(0).to(*args, **kwargs).device          # moves, never casts
+        device = self.values[:0].to(*args, **kwargs).device         # moves, never casts
         return TopLogits(self.values.to(device), self.indices.to(device), None if self.rest is None else self.rest.to(device),
                          self.temperature)
 
@@ -199,7 +204,7 @@ def top_logits(logits, k, temperature=1.0):
     if logits.dim() != 2 or logits.shape[1] < 1:
         raise ValueError('logits must be [rows, classes] with a class at least: got {}'.format(tuple(logits.shape)))
     rows, classes = logits.shape
-    k = int(k)
+    k = operator.index(k)
     if not 1 <= k <= min(MAX_K, classes):
         raise ValueError('k is {}: 1 to {} of {} classes can be listed'.format(k, min(MAX_K, classes), classes))
     return TopLogits(*_ext().top_logits(logits, k, temperature), temperature)

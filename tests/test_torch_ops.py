@@ -647,6 +647,135 @@ def test_captured_backward_beside_an_eager_graph():
     assert torch.equal(got, want)
 
 
+# ---- calls that are allowed and unusual ---------------------------------------------------------------------------------
+@gpu
+def test_captured_backward_of_what_a_leaf_was_made_into():
+    """the leaf behind a view, a cast or a layer counts as well"""
+    p = to_gpu(problem(1, 20, 1, 8, 8, 'f32', seed=14))
+    leaf = p['q'].requires_grad_()
+    call = lambda: ops.decay_attention(leaf * 2, p['k'], p['v'], p['log_decay'])                   # noqa: E731
+    eager = call()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match='alive'):
+        with torch.cuda.graph(graph):
+            call()
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(eager, leaf, p['grad_out'])[0]
+    x, teacher, weight = distill_problem(3, 70, 9, 'f32', 2.0, seed=14)
+    x, teacher, weight = x.cuda().requires_grad_(), teacher.to('cuda'), weight.cuda()
+    eager = ops.distillation_loss(x.view(3, 70), teacher, weight)
+    with pytest.raises(RuntimeError, match='alive'):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.distillation_loss(x.view(3, 70), teacher, weight)
+    torch.cuda.synchronize()
+    del eager, graph
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(call(), leaf, p['grad_out'])[0]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_what_autograd_refuses():
+    p = to_gpu(problem(2, 20, 1, 8, 8, 'f32', False, True, seed=15))
+    args = [p[n] for n in ARGS]
+    args[0].requires_grad_()
+    out = ops.decay_attention(*args)
+    with pytest.raises(NotImplementedError, match='second derivative'):
+        torch.autograd.grad(out.sum(), args[0], create_graph=True)
+    out = ops.decay_attention(*args)
+    args[1].add_(1.0)                                              # k is needed as it was
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        out.sum().backward()
+    x, teacher, weight = distill_problem(3, 7, 2, 'f32', 2.0, seed=15)
+    x, teacher, weight = x.cuda().requires_grad_(), teacher.to('cuda'), weight.cuda()
+    with pytest.raises(NotImplementedError, match='second derivative'):
+        torch.autograd.grad(ops.distillation_loss(x, teacher, weight), x, create_graph=True)
+    loss = ops.distillation_loss(x, teacher, weight)
+    teacher.indices.zero_()
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+
+
+@gpu
+def test_inference_mode_and_twice_backward():
+    with torch.inference_mode():
+        p = to_gpu(problem(2, 3, 2, 16, 8, 'bf16', False, True, seed=16))
+        whole, last = ops.decay_attention(*[p[n] for n in ARGS], return_state=True)
+        state = p['initial_state'].clone()
+        for t in range(3):
+            row = ops.decay_attention_step(p['q'][:, t], p['k'][:, t], p['v'][:, t], p['log_decay'], state)
+            assert float((row - whole[:, t]).abs().max()) <= 2.0**-7 * float(whole[:, t].abs().max())     # two roundings
+        # both sum the same products in float32 in their own order: a few of 2^-24 of the largest terms
+        assert torch.allclose(state, last, rtol=1e-5, atol=1e-5 * float(last.abs().max()))
+    p = to_gpu(problem(2, 30, 2, 16, 8, 'f32', seed=16))
+    q = p['q'].requires_grad_()
+    out = ops.decay_attention(q, p['k'], p['v'], p['log_decay'])
+    one = torch.autograd.grad(out, q, p['grad_out'], retain_graph=True)[0]
+    assert torch.equal(one, torch.autograd.grad(out, q, p['grad_out'])[0])
+
+
+@gpu
+def test_threads_with_streams_of_their_own():
+    """eight threads, each with its own stream and sizes, forward and backward at once: every one gets what it gets alone"""
+    import threading
+
+    def work(n, results):
+        p = to_gpu(problem(1 + n, 100 + 50 * n, 2, 16 * (n % 3 + 1), 32, ('f32', 'bf16', 'f16')[n % 3], seed=20 + n))
+        x, teacher, weight = distill_problem(20 + n, 300 + 400 * n, 9, 'f32', 2.0, seed=20 + n)
+        x, teacher, weight = x.cuda().requires_grad_(), teacher.to('cuda'), weight.cuda()
+        q = p['q'].requires_grad_()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            for _ in range(5):
+                out = ops.decay_attention(q, p['k'], p['v'], p['log_decay'], p.get('lengths'))
+                grad = torch.autograd.grad(out, q, p['grad_out'])[0]
+                loss = ops.distillation_loss(x, teacher, weight)
+                g = torch.autograd.grad(loss, x)[0]
+                top = ops.top_logits(x.detach(), 9)
+            stream.synchronize()
+            results[n] = [y.detach().cpu() for y in (out, grad, loss, g, top.values, top.indices, top.rest)]
+    alone, together = {}, {}
+    for n in range(8):
+        work(n, alone)
+    threads = [threading.Thread(target=work, args=(n, together)) for n in range(8)]
+    [t.start() for t in threads], [t.join() for t in threads]
+    for n in range(8):
+        for y, z in zip(together[n], alone[n]):
+            assert torch.equal(y, z), n
+
+
+@gpu
+@pytest.mark.parametrize('rows,classes,k', [(500, 5000, 64), (300, 900, 20), (100, 60001, 128)])
+def test_top_logits_gives_the_same_bits_again(rows, classes, k):
+    """nothing depends on the order in which threads note what they find"""
+    x = torch.randn(rows, classes, generator=torch.Generator().manual_seed(3)).cuda()
+    first = ops.top_logits(x, k, 0.7)
+    for _ in range(20):
+        again = ops.top_logits(x, k, 0.7)
+        for name in ('values', 'indices', 'rest'):
+            assert torch.equal(getattr(first, name), getattr(again, name)), name
+
+
+@gpu
+def test_more_rows_than_one_axis_of_a_grid_holds():
+    rows = (1 << 26) + 5                                           # four to a workgroup of 256: 2^32 threads and more
+    x = torch.randn(rows, 2, device='cuda', generator=torch.Generator('cuda').manual_seed(4))
+    t = ops.top_logits(x, 1)
+    want, at = x.max(dim=1)
+    assert torch.equal(t.values[:, 0], want) and torch.equal(t.indices[:, 0], at.int())
+    assert torch.allclose(t.rest, x.min(dim=1).values, rtol=1e-6, atol=1e-6)
+    student = torch.stack([x[:, 1], x[:, 0]], dim=1)
+    loss, grad = ops.distillation_loss_and_gradient(student, t, reduction='none')
+    for part in (slice(0, 1000), slice((1 << 26) - 500, rows)):    # softmaxes of two, in 64 bits
+        p, q = x[part].double().log_softmax(1), student[part].double().log_softmax(1)
+        assert torch.allclose(loss[part].double(), (p.exp() * (p - q)).sum(1), rtol=1e-5, atol=1e-6)
+        assert torch.allclose(grad[part].double(), q.exp() - p.exp(), rtol=1e-5, atol=1e-6)
+
+
 # ---- refusals (on the CPU: nothing is launched) -------------------------------------------------------------------------
 @pytest.fixture
 def dry(monkeypatch):
@@ -781,3 +910,27 @@ def test_structs_match_the_header():
         subprocess.check_call(['gcc', '-I' + os.path.join(root, 'include'), os.path.join(d, 'sz.c'), '-o', exe])
         sizes = [int(v) for v in subprocess.check_output([exe]).split()]
     assert sizes == [C.sizeof(N.PxgSequence), C.sizeof(N.PxgDecay), C.sizeof(N.PxgDistill)]
+
+
+def test_more_pairs_than_a_grid_holds(dry):
+    """refused by the checks and by the C entries (views of one element: nothing of that size exists)"""
+    q = torch.zeros(1, 1, 1, 1).expand(1 << 22, 1, 2, 1)
+    with pytest.raises(ValueError, match='at most'):
+        ops.decay_attention(q, q, q, torch.zeros(2))
+    s = N.PxgDecay()
+    s.struct_bytes, s.batch, s.steps, s.heads, s.dk, s.dv = C.sizeof(s), 1 << 22, 1, 2, 1, 1
+    lib = N.load_library()
+    assert lib.pxg_decay_workspace_bytes(C.byref(s), 0) == -1
+    s.batch -= 1
+    assert lib.pxg_decay_workspace_bytes(C.byref(s), 0) == 0
+    s.batch, s.heads = 0, 1 << 24
+    assert lib.pxg_decay_workspace_bytes(C.byref(s), 0) == -1
+
+
+def test_answers_are_moved_never_cast():
+    t = ops.TopLogits(torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int32), torch.zeros(3), 2.0)
+    for to in (torch.float16, 'cpu', torch.device('cpu'), torch.empty(1, dtype=torch.float64)):
+        moved = t.to(to)
+        assert moved.values.dtype == torch.float32 and moved.indices.dtype == torch.int32 and moved.temperature == 2.0
+    meta = ops.TopLogits(torch.zeros(3, 2, device='meta'), torch.zeros(3, 2, dtype=torch.int32, device='meta')).to(torch.float16)
+    assert meta.values.device.type == 'meta'
