@@ -36,6 +36,13 @@ __device__ __forceinline__ int64_t decay_length(const DecayRuns& s, int b)
     return n < 0 ? 0 : n > s.steps ? s.steps : n;
 }
 
+// exp(n log_a): what the product's rounding takes is given back, for it would be the same in every chunk
+__device__ __forceinline__ float decay_over(float n, float log_a)
+{
+    const float p = n * log_a, lost = fmaf(n, log_a, -p), w = expf(p);
+    return w > 0.f && w < INFINITY ? fmaf(w, lost, w) : w;
+}
+
 // steps in a chunk, by the type's number of bfloat16 planes and the padded width
 constexpr int decay_chunk(int dtype, int width)
 {

@@ -26,7 +26,7 @@ __global__ __launch_bounds__(256) void k_decay_join(const DecayRuns a, int chunk
     const int i = blockIdx.y * 256 + threadIdx.x;
     if (i >= size) return;
     const int used = (int)((uint32_t)(decay_length(a, (int)bh / a.heads) + chunk - 1) / (uint32_t)chunk);
-    const float steps = (float)a.segment_chunks * (float)chunk, decay = expf(steps * a.log_decay[(int)bh % a.heads]);
+    const float steps = (float)a.segment_chunks * (float)chunk, decay = decay_over(steps, a.log_decay[(int)bh % a.heads]);
     const bool slope = (int)blockIdx.z < slope_runs;
     float* c = r.carry + bh * n * size + i;
     float S = c[0], G = slope ? c[slopes] : 0.f;

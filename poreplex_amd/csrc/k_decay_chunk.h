@@ -224,6 +224,7 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
     constexpr int PROW = C + 8, PPLANE = C * PROW;            // of the weights
     constexpr int SLOPE_PLANES = 3;
     constexpr bool OUT = !STATES_ONLY, DOT = SLOPE && OUT;
+    constexpr int KEEP_S = DOT ? 2 : KEEP;                    // of the state against x: the gradient of log_decay is made of them, too
     static_assert(PIECES * N == C * (D / 8), "whole pieces");
     const int bh = xcd_order(blockIdx.x, gridDim.x), b = bh / a.heads, h = bh % a.heads, seg = blockIdx.y;
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, g = lane / 16, li = lane % 16, f0 = wave * 16;
@@ -247,7 +248,7 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
     }
 
     const float log_a = a.log_decay[h];
-    for (int n = tid; n <= C; n += N) pw[n] = n ? expf((float)n * log_a) : 1.f;
+    for (int n = tid; n <= C; n += N) pw[n] = n ? decay_over((float)n, log_a) : 1.f;
     if (tid < 2) strange[tid] = 0;
     __syncthreads();
     // factors of one lane: inside a diagonal tile, for tiles further off, for the state (index: step 4 g + s of a tile)
@@ -455,7 +456,7 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
             }
 #pragma unroll
             for (int k = 0; k < KB; k++) {
-                Operand su[KEEP + 1], gu[SLOPE ? SLOPE_PLANES : 1];
+                Operand su[KEEP_S + 1], gu[SLOPE ? SLOPE_PLANES : 1];
                 const auto operand = [&](const f32x4* of, auto planes, Operand* to) {
                     constexpr int M = decltype(planes)::value;
                     bf16x4 u[M], v[M];
@@ -469,14 +470,14 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
                         for (int p = 0; p < M; p++) to[p] = u[p];
                     }
                 };
-                operand(S, std::integral_constant<int, KEEP + 1>(), su);
+                operand(S, std::integral_constant<int, KEEP_S + 1>(), su);
                 if constexpr (DOT) operand(G, std::integral_constant<int, SLOPE_PLANES>(), gu);
 #pragma unroll
                 for (int it = 0; it < CT; it++) {
                     Operand xb[NP];
 #pragma unroll
                     for (int p = 0; p < NP; p++) xb[p] = block(tx, it, k, p);
-                    o[it] = plane_products<KEEP + 1, NP, KEEP>(su, xb, o[it]);
+                    o[it] = plane_products<KEEP_S + 1, NP, KEEP_S>(su, xb, o[it]);
                     if constexpr (DOT) d[it] = plane_products<SLOPE_PLANES, NP, SLOPE_PLANES - 1>(gu, xb, d[it]);
                 }
             }
