@@ -376,6 +376,38 @@ def check_top(x, k, temperature):
 
 
 @gpu
+@pytest.mark.parametrize('dtype', sorted(TYPES))
+@pytest.mark.parametrize('rows,classes,k', [(1, 2, 1), (33, 8, 8), (65, 9, 4), (17, 16, 1), (9, 17, 17), (5, 32, 31), (7, 33, 3), (6, 64, 64),
+                                            (6, 65, 64)])
+def test_top_logits_of_few_classes(rows, classes, k, dtype):
+    g = torch.Generator().manual_seed(classes + k)
+    x = (torch.randn(rows, classes + 3, generator=g) * 3).to(TYPES[dtype])
+    x[-1] = torch.randint(0, 3, (classes + 3,), generator=g).to(TYPES[dtype])
+    check_top(x[:, :classes].contiguous(), k, 1.5)
+    t, u = ops.top_logits(x.cuda()[:, 2:-1], k, 1.5), ops.top_logits(x[:, 2:-1].contiguous().cuda(), k, 1.5)     # not aligned
+    for name in ('values', 'indices', 'rest'):
+        assert torch.equal(getattr(t, name), getattr(u, name))
+
+
+@gpu
+def test_top_logits_strange_rows_of_few_classes():
+    inf, nan = math.inf, math.nan
+    for classes in (5, 40):
+        x = torch.zeros(9, classes)
+        x[0] = -inf
+        x[1, 2:] = -inf
+        x[2, 3] = inf
+        x[3, 1:] = inf
+        x[4, 4] = nan
+        x[5] = torch.arange(float(classes))
+        x[6, :4] = nan
+        x[7, ::2] = -0.0
+        x[8] = torch.finfo(torch.float32).min
+        for k in (1, 2, 5):
+            check_top(x, k, 1.0)
+
+
+@gpu
 def test_top_logits_strange_rows():
     inf, nan = math.inf, math.nan
     x = torch.zeros(9, 300)
