@@ -414,7 +414,7 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
 }
 
 // Rows of up to 64 classes: a lane for each of them, so that nothing is noted or searched for; an element's place is the number of
-// those ahead of it.   10 000 x 5 f32, k = 3: 3.6 us, with a wave for a row 8.5.
+// those ahead of it.  10 000 x 5 f32, k = 3: 3.6 us, with a wave for a row 8.5.
 template <int G, typename T>
 __global__ __launch_bounds__(256)
 void k_top_narrow(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, int k, float temperature, T* values,
