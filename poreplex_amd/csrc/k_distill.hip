@@ -11,6 +11,10 @@
 //
 // All of them are bound by reading the logits once (and writing the gradient once): a row belongs to one wave, to four or to
 // sixteen, by its length and the number of rows, and every lane reads 16 bytes at a time, four times before it computes.
+//   4 096 x 32 768 bf16, k = 32:      loss 75 us (3.6 TB/s), gradient 90 (6.0)
+//   1 023 x 131 071 f32, k = 100:     loss 108 to 147 (5.0 to 3.6), gradient 211 (5.1), where a copy of 2 GiB reaches 4.9
+//   2 047 x 50 001 bf16, k = 64:      the largest logits 72 (2.8): exponentials and comparisons fill the other half of the time
+//   10 000 x 5 f32 and 256 x 5 f32:   3.6, and 10 + 2 + 4.4: launches and the latency of a few dependent reductions
 #include "pxg_ops.h"
 #include <type_traits>
 
