@@ -138,7 +138,7 @@ def parse(argv=None):
     ap.add_argument('--strong-base-reads', type=int, default=2048,
                     help='distinct reads of the configs4_strong leg (tiled on the device)')
     ap.add_argument('--no-worker-processes-leg', action='store_true',
-                    help='API leg: skip the 128-read calls from 8 / 16 worker PROCESSES (the reference\'s ProcessPoolExecutor pattern)')
+                    help='API leg: skip the 128-read calls from 8 / 14 worker PROCESSES (the reference\'s ProcessPoolExecutor pattern)')
     ap.add_argument('--no-latency-leg', action='store_true',
                     help='skip the small-batch leg (roofline.latency_form: a 1 024-read batch with and without the latency forms of K2 / K5)')
     return ap.parse_args(argv)
@@ -561,14 +561,15 @@ def fast5_calls_leg(args, base, which, lo, mask, local_rank, resident_records, n
         shutil.rmtree(work, ignore_errors=True)
 
 
-def worker_processes_leg(args, base, which, lo, mask, local_rank, workers=(8, 16), calls_per_worker=40, n=128):
+def worker_processes_leg(args, base, which, lo, mask, local_rank, workers=(8, 14), calls_per_worker=40, n=128):
     """The reference's OWN call pattern for its per-read processor (pipeline.py:96,193-205): a ProcessPoolExecutor of
     `parallel` worker processes, each running process_batch(batchid, reads, config) on 128-read batches
     (commandline.py:402) and handing the list of result dicts back through the executor's pipe.  Every worker process
     has its own interpreter and its own context on the ONE GPU (WorkerPersistenceStorage in that process); a
     128-read batch takes the latency forms of the LSTM kernels on 32 of the 256 CUs, so the workers' kernels run side by
     side.  Every worker builds its context in the pool's initializer and 20 x workers warm-up calls are served before the
-    clock starts; timed: `calls_per_worker` x workers calls submitted at once, the result lists arriving in the parent
+    clock starts (fifteen processes with the parent: a machine may bound those that use one GPU at sixteen); timed:
+    `calls_per_worker` x workers calls submitted at once, the result lists arriving in the parent
     (pickling included)."""
     import multiprocessing as mp
     import shutil
