@@ -808,6 +808,58 @@ def test_more_rows_than_one_axis_of_a_grid_holds():
         assert torch.allclose(grad[part].double(), q.exp() - p.exp(), rtol=1e-5, atol=1e-6)
 
 
+@gpu
+def test_offsets_beyond_32_bits():
+    """rows behind the 2^31st element are computed as they are alone (the same kernels on the same numbers: the same bits, or, where
+    an earlier memory of exp(-2000) is left out or the time axis is cut elsewhere, two roundings of the result)"""
+    g = torch.Generator('cuda').manual_seed(5)
+    normal = lambda *shape, dtype=torch.bfloat16: torch.randn(*shape, device='cuda', dtype=dtype, generator=g)          # noqa: E731
+    steps, tail = (1 << 20) + 77, 2048                             # 16 heads of 128: 2^31 elements and more
+    q, k, v, go = (normal(1, steps, 16, 128) for _ in range(4))
+    log_decay = torch.full((16,), -1.0, device='cuda')
+
+    def last(t):
+        return t[:, -tail:].contiguous()
+    out = ops.decay_attention(q, k, v, log_decay)
+    near = lambda x, y: bool(((x.float() - y.float()).abs() <= 2.0**-7 * y.float().abs() + 2.0**-9 * y.float().abs().max()).all())  # noqa: E731
+    alone = ops.decay_attention(last(q), last(k), last(v), log_decay)
+    assert near(out[:, -1000:], alone[:, -1000:])
+    del out
+    grads = ops.decay_attention_backward(go, q, k, v, log_decay)[:3]
+    alone = ops.decay_attention_backward(last(go), last(q), last(k), last(v), log_decay)[:3]
+    for x, y in zip(grads, alone):
+        assert near(x[:, -1000:], y[:, -1000:])
+    del q, k, v, go, grads
+    # sequences that lie so far apart, and steps of a stride that no 32-bit offset inside a chunk holds
+    store = torch.empty((1 << 31) + (1 << 20), device='cuda', dtype=torch.bfloat16)
+    p = to_gpu(problem(2, 70, 2, 64, 64, 'bf16', True, seed=6))
+    want = ops.decay_attention(p['q'], p['k'], p['v'], p['log_decay'], p['lengths'])
+    far = store.as_strided((2, 70, 2, 64), (1 << 31, 128, 64, 1))
+    far.copy_(p['k'])
+    assert torch.equal(ops.decay_attention(p['q'], far, p['v'], p['log_decay'], p['lengths']), want)
+    apart = store.as_strided((2, 70, 2, 64), (128, 1 << 24, 64, 1))
+    apart.copy_(p['v'])
+    assert torch.equal(ops.decay_attention(p['q'], p['k'], apart, p['log_decay'], p['lengths']), want)
+    del store, far, apart
+    # many states, many logits
+    pairs = 131072 + 3
+    state, first = torch.empty(pairs, 1, 128, 128, device='cuda').normal_(generator=g), normal(3, 1, 128)
+    one = state[-3:].clone()
+    x = first[:1].expand(pairs, 1, 128).clone()
+    x[-3:] = first
+    got = ops.decay_attention_step(x, x, x, log_decay[:1], state)
+    assert torch.equal(got[-3:], ops.decay_attention_step(first, first, first, log_decay[:1], one)) and torch.equal(state[-3:], one)
+    del state, x, got
+    rows = (1 << 16) + 300
+    logits = normal(rows, 32768)
+    t = ops.top_logits(logits, 20)
+    end = ops.top_logits(logits[-300:].contiguous(), 20)
+    assert torch.equal(t.values[-300:], end.values) and torch.equal(t.indices[-300:], end.indices) and torch.equal(t.rest[-300:], end.rest)
+    loss, grad = ops.distillation_loss_and_gradient(logits, ops.TopLogits(t.values * 2, t.indices, t.rest), None, 'none')
+    end = ops.distillation_loss_and_gradient(logits[-300:].contiguous(), ops.TopLogits(end.values * 2, end.indices, end.rest), None, 'none')
+    assert torch.equal(loss[-300:], end[0]) and torch.equal(grad[-300:], end[1])
+
+
 # ---- refusals (on the CPU: nothing is launched) -------------------------------------------------------------------------
 @pytest.fixture
 def dry(monkeypatch):
