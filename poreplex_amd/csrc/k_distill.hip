@@ -499,17 +499,18 @@ template <int G> struct LossShared {
     double share[PXG_TOP_MAX_K];
     double redd[G / 64];
     float redf[G / 64];
-    int red[G / 64];
 };
 
 // `stats` of a row: the unlisted classes' maximum, the factor of their exponentials in the gradient, whether the row counts (0: no,
 // 1: yes, NaN: it names what is no class), unused, then q - p of each place (+inf: no class's first place)
 constexpr int STATS = 4;
 
+// The classes are everybody's; what there is one of for each listed class, and every sum over those, is the first wave's, which
+// needs no barrier for it (with the whole workgroup at eight such sums a row of 2 000 classes took twice as long).
 template <int G, typename T>
 __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_forward(const pxg_distill a)
 {
-    constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n, PLACES = (PXG_TOP_MAX_K + G - 1) / G;
+    constexpr int GROUPS = G == 64 ? 4 : 1, n = Unit<T>::n, PLACES = PXG_TOP_MAX_K / 64;
     __shared__ LossShared<G> shared[GROUPS];
     const int64_t row = row_of<G>();
     if (row >= a.rows) return;
@@ -518,60 +519,30 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_forward(const pxg
     float* stats = a.stats + row * (STATS + k);
     const double w = a.weight ? (double)a.weight[row] : 1.0, tau = a.temperature;
     const T* x = (const T*)a.logits + row * a.row_stride;
-
-    // the teacher's shares
-    s.marks.clear(t);
-    int bad = 0;
-    double value[PLACES], most = -INFINITY;
-#pragma unroll
-    for (int p = 0; p < PLACES; p++) {
-        const int i = t + p * G;
-        value[p] = -INFINITY;
-        if (i < k) {
-            const int64_t at = row * k + i;
-            int64_t index = a.indices_are_64 ? ((const int64_t*)a.indices)[at] : ((const int32_t*)a.indices)[at];
-            if (index < -1 || index >= a.classes) bad = 1, index = -1;
-            if (index >= 0) value[p] = number_at(a.values, at, a.value_dtype) / tau;
-            s.index[i] = (int32_t)index;
-            most = value[p] > most ? value[p] : most;
-        }
-    }
-    const double rest = a.rest ? (double)a.rest[row] : -INFINITY;
-    bad = group_reduce<G>(bad, s.red, MaxOf());
-    double top = group_reduce<G>(most, s.redd, MaxOf());
-    top = rest > top ? rest : top;
-    double sum = 0.0;
-#pragma unroll
-    for (int p = 0; p < PLACES; p++) {
-        value[p] = value[p] == -INFINITY ? 0.0 : exp(value[p] - top);
-        sum += value[p];
-    }
-    const double rest_exp = rest == -INFINITY ? 0.0 : exp(rest - top);
-    const double total_p = group_reduce<G>(sum, s.redd, SumOf()) + rest_exp;
-    if (w == 0.0 || (total_p == 0.0 && !bad)) {                   // the whole group
+    if (w == 0.0) {                                               // the whole group
         if (t == 0) stats[2] = 0.f, a.row_loss[row] = 0.f;
         return;
     }
-    const double p_rest = rest_exp / total_p;
-#pragma unroll
-    for (int p = 0; p < PLACES; p++)
-        if (t + p * G < k) s.share[t + p * G] = value[p] / total_p;
+    s.marks.clear(t);
     group_sync<G>();
-    // a class that is listed more than once: its first place takes all its shares
-    double share[PLACES];
-    bool first[PLACES];
+    double value[PLACES], xi[PLACES], rest = -INFINITY;
+    int32_t index[PLACES];
+    bool bad = false;
+    if (t < 64) {
+        rest = a.rest ? (double)a.rest[row] : -INFINITY;
 #pragma unroll
-    for (int p = 0; p < PLACES; p++) {
-        const int i = t + p * G;
-        const int32_t index = i < k ? s.index[i] : -1;
-        share[p] = 0.0, first[p] = index >= 0;
-        if (index >= 0) {
-            for (int j = 0; j < k; j++)
-                if (s.index[j] == index) {
-                    if (j < i) first[p] = false;
-                    share[p] += s.share[j];
-                }
-            s.marks.add(index, n);
+        for (int p = 0; p < PLACES; p++) {
+            const int i = t + p * 64;
+            value[p] = xi[p] = -INFINITY, index[p] = -1;
+            if (i >= k) continue;
+            const int64_t at = row * k + i, is = a.indices_are_64 ? ((const int64_t*)a.indices)[at] : ((const int32_t*)a.indices)[at];
+            if (is < -1 || is >= a.classes) bad = true;
+            else index[p] = (int32_t)is;
+            s.index[i] = index[p];
+            if (index[p] < 0) continue;
+            s.marks.add(index[p], n);
+            value[p] = number_at(a.values, at, a.value_dtype) / tau;
+            xi[p] = (double)pxg_to_f32(x[index[p]]);
         }
     }
     group_sync<G>();
@@ -608,19 +579,66 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_forward(const pxg
         for (int e = 0; e < n; e++) next = larger(next, v[e]);
         sum_u.add(v, next, scale);
     });
-    const float all_u = group_reduce<G>(sum_u.base, s.redf, MaxOf());
-    // (a thread without any keeps its sum of 0 whatever its exponent says)
-    const double unlisted = group_reduce<G>(sum_u.sum == 0.f ? 0.0 : (double)sum_u.sum * (double)exp_from<T>(sum_u.base, all_u, scale),
-                                                s.redd, SumOf());
+    // (what has none keeps its sum of 0 whatever its exponent says)
+    float all_u = group_reduce<64>(sum_u.base, s.redf, MaxOf());
+    double unlisted = group_reduce<64>(sum_u.sum == 0.f ? 0.0 : (double)sum_u.sum * (double)exp_from<T>(sum_u.base, all_u, scale),
+                                       s.redd, SumOf());
+    if constexpr (G > 64) {
+        if (t % 64 == 0) s.redf[t / 64] = all_u, s.redd[t / 64] = unlisted;
+        __syncthreads();
+        if (t >= 64) return;
+        const float most = t < G / 64 ? s.redf[t] : -INFINITY;
+        const double sum = t < G / 64 ? s.redd[t] : 0.0;
+        all_u = group_reduce<64>(most, s.redf, MaxOf());
+        unlisted = group_reduce<64>(sum == 0.0 ? 0.0 : sum * (double)exp_from<T>(most, all_u, scale), s.redd, SumOf());
+    }
 
-    // the k + 1 shares
-    double xi[PLACES], base = -INFINITY;
+    // the first wave.  The teacher's shares
+    bad = __any(bad);
+    double most = -INFINITY, sum = 0.0;
+#pragma unroll
+    for (int p = 0; p < PLACES; p++) most = value[p] > most ? value[p] : most;
+    double top = group_reduce<64>(most, s.redd, MaxOf());
+    top = rest > top ? rest : top;
 #pragma unroll
     for (int p = 0; p < PLACES; p++) {
-        xi[p] = first[p] ? (double)pxg_to_f32(x[s.index[t + p * G]]) : -INFINITY;
+        value[p] = value[p] == -INFINITY ? 0.0 : exp(value[p] - top);
+        sum += value[p];
+    }
+    const double rest_exp = rest == -INFINITY ? 0.0 : exp(rest - top);
+    const double total_p = group_reduce<64>(sum, s.redd, SumOf()) + rest_exp;
+    if (total_p == 0.0 && !bad) {
+        if (t == 0) stats[2] = 0.f, a.row_loss[row] = 0.f;
+        return;
+    }
+    const double p_rest = rest_exp / total_p;
+#pragma unroll
+    for (int p = 0; p < PLACES; p++)
+        if (t + p * 64 < k) s.share[t + p * 64] = value[p] / total_p;
+    group_sync<64>();
+    // a class that is listed more than once: its first place takes all its shares
+    double share[PLACES];
+    bool first[PLACES];
+#pragma unroll
+    for (int p = 0; p < PLACES; p++) {
+        const int i = t + p * 64;
+        share[p] = 0.0, first[p] = index[p] >= 0;
+        if (index[p] >= 0)
+            for (int j = 0; j < k; j++)
+                if (s.index[j] == index[p]) {
+                    if (j < i) first[p] = false;
+                    share[p] += s.share[j];
+                }
+    }
+
+    // the k + 1 shares
+    double base = -INFINITY;
+#pragma unroll
+    for (int p = 0; p < PLACES; p++) {
+        if (!first[p]) xi[p] = -INFINITY;
         base = xi[p] > base ? xi[p] : base;
     }
-    base = group_reduce<G>(base, s.redd, MaxOf());
+    base = group_reduce<64>(base, s.redd, MaxOf());
     if (unlisted != 0.0 && !((double)all_u <= base)) base = all_u;
     double listed = 0.0;
 #pragma unroll
@@ -630,15 +648,15 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_forward(const pxg
     }
     const double far_u = ((double)all_u - base) / tau;
     const double u = unlisted == 0.0 ? 0.0 : unlisted * exp(far_u);
-    const double total = group_reduce<G>(listed, s.redd, SumOf()) + u, log_total = log(total);
+    const double total = group_reduce<64>(listed, s.redd, SumOf()) + u, log_total = log(total);
     double term = 0.0;
 #pragma unroll
     for (int p = 0; p < PLACES; p++) {
-        const int i = t + p * G;
+        const int i = t + p * 64;
         if (first[p] && share[p] != 0.0) term += share[p] * (log(share[p]) - (xi[p] - log_total));
         if (i < k) stats[STATS + i] = first[p] ? (float)(exp(xi[p]) / total - share[p]) : INFINITY;
     }
-    double loss = group_reduce<G>(term, s.redd, SumOf());
+    double loss = group_reduce<64>(term, s.redd, SumOf());
     if (t == 0) {
         if (p_rest != 0.0) loss += p_rest * (log(p_rest) - (log(unlisted) + far_u - log_total));
         if (bad) loss = NAN;
@@ -722,9 +740,12 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_backward(const px
 
 // The threads that share a row: a wave for short ones, a workgroup of four waves, sixteen where there are too few long rows to
 // fill the card with less (one row of 131 071 f32, loss and gradient: 70 us with four, 48 with sixteen; 400 rows: 148 and 154).
-int threads_of(int64_t rows, int64_t classes)
+// Many rows of up to 16 KB are better off with a wave each, too (16 384 rows, loss and gradient with one wave / four: 1 200 f16 79 /
+// 112 us, 5 000 f16 150 / 170, 8 000 f16 217 / 218, 5 000 f32 258 / 230; 2 048 x 3 305 f16 29 / 27, 512 rows 23 / 18).
+int threads_of(int64_t rows, int64_t classes, size_t element)
 {
-    return classes <= 1024 ? 64 : rows < 256 && classes > 16384 ? 1024 : 256;
+    if (classes <= 1024 || (rows >= 4096 && classes * (int64_t)element <= 16384)) return 64;
+    return rows < 256 && classes > 16384 ? 1024 : 256;
 }
 
 dim3 blocks_of(int64_t rows, int threads)
@@ -746,8 +767,11 @@ void launch_top(int64_t rows, int64_t classes, const void* logits, int64_t row_s
     if (classes <= 16) return narrow(std::integral_constant<int, 16>());
     if (classes <= 32) return narrow(std::integral_constant<int, 32>());
     if (classes <= 64) return narrow(std::integral_constant<int, 64>());
-    int g = threads_of(rows, classes);
-    if (k > 32 && g == 64) g = 256;                               // twice as many threads as are to be chosen
+    // a wave holds up to 32 (twice as many threads as are to be chosen), and serves many rows of up to 64 KB better than a workgroup
+    // each (k = 4, four waves / one: 2 048 x 5 000 f32 22 / 14 us, 16 384 x 16 000 f16 159 / 110, 16 384 x 16 000 f32 201 / 188,
+    // 16 384 x 32 000 f32 354 / 364, 1 024 x 5 000 f16 12 / 11, 256 x 5 000 f32 11 / 11, 256 x 16 000 f32 14 / 19)
+    const bool one_wave = k <= 32 && (classes <= 1024 || (rows >= 2048 && classes * (int64_t)sizeof(T) <= 65536));
+    const int g = one_wave ? 64 : rows < 256 && classes > 16384 ? 1024 : 256;
     const dim3 blocks = blocks_of(rows, g);
     switch (g) {
     case 64: k_top<64, T><<<blocks, 256, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest); break;
@@ -758,7 +782,7 @@ void launch_top(int64_t rows, int64_t classes, const void* logits, int64_t row_s
 
 template <typename T> void launch_forward(const pxg_distill& a, hipStream_t st)
 {
-    const int g = threads_of(a.rows, a.classes);
+    const int g = threads_of(a.rows, a.classes, sizeof(T));
     const dim3 blocks = blocks_of(a.rows, g);
     switch (g) {
     case 64: k_distill_forward<64, T><<<blocks, 256, 0, st>>>(a); break;
@@ -769,7 +793,7 @@ template <typename T> void launch_forward(const pxg_distill& a, hipStream_t st)
 
 template <typename T> void launch_backward(const pxg_distill& a, hipStream_t st)
 {
-    const int g = threads_of(a.rows, a.classes);
+    const int g = threads_of(a.rows, a.classes, sizeof(T));
     const dim3 blocks = blocks_of(a.rows, g);
     switch (g) {
     case 64: k_distill_backward<64, T><<<blocks, 256, 0, st>>>(a); break;

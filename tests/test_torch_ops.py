@@ -679,6 +679,42 @@ def test_captured_backward_beside_an_eager_graph():
     assert torch.equal(got, want)
 
 
+@gpu
+@pytest.mark.parametrize('rows,classes,k,dtype', [(2050, 5003, 31, 'f32'), (2048, 5001, 32, 'bf16'), (4097, 1031, 1, 'f16')])
+def test_top_logits_of_many_rows(rows, classes, k, dtype):
+    """a wave for each row, however long"""
+    inf, nan = math.inf, math.nan
+    g = torch.Generator().manual_seed(classes)
+    x = torch.randn(rows, classes, generator=g) * 3
+    x[0], x[1], x[2] = -inf, torch.arange(float(classes)), -torch.arange(float(classes))
+    x[3, 5:] = -inf
+    x[4, 7], x[5, 100:140], x[6, 900], x[7] = inf, inf, nan, 1.0
+    x[8] = torch.arange(classes) // 64 % 7
+    x[9] = torch.finfo(TYPES[dtype]).min
+    x[10, 3:40] = nan
+    x[-1] = torch.randint(0, 3, (classes,), generator=g).float()
+    check_top(x.to(TYPES[dtype]), k, 1.0)
+
+
+@gpu
+@pytest.mark.parametrize('rows,classes,k,dtype', [(4096, 2047, 5, 'f32'), (4099, 1500, 100, 'bf16')])
+def test_distillation_loss_of_many_rows(rows, classes, k, dtype):
+    """a wave for each row, against a workgroup for each row of a part of them: both within a few roundings of float32 of the same
+    loss, and of gradients that are rounded to their type"""
+    x, teacher, weight = distill_problem(rows, classes, k, dtype, 2.0, seed=30)
+    x, teacher, weight = x.cuda(), teacher.to('cuda'), weight.cuda()
+    loss, grad = ops.distillation_loss_and_gradient(x, teacher, weight, 'none')
+    for part in (slice(0, 700), slice(rows - 700, rows)):
+        one, g = ops.distillation_loss_and_gradient(x[part], teacher[part], weight[part], 'none')
+        assert torch.allclose(loss[part], one, rtol=1e-5, atol=1e-5 * float(one.abs().max()))
+        assert torch.allclose(grad[part].float(), g.float(), rtol=1e-5 + torch.finfo(g.dtype).eps, atol=1e-6 * float(g.float().abs().max()))
+    want, gradient = distill_statement(*[y.double().cpu().numpy() for y in (x[-40:], teacher.values[-40:])],
+                                       teacher.indices[-40:].cpu().numpy(), None if teacher.rest is None else teacher.rest[-40:].double().cpu().numpy(),
+                                       2.0, weight[-40:].double().cpu().numpy())[:2]
+    assert np.allclose(loss[-40:].double().cpu().numpy(), want, rtol=1e-4, atol=1e-4 * np.abs(want).max())
+    assert np.allclose(grad[-40:].double().cpu().numpy(), gradient, rtol=1e-4 + torch.finfo(grad.dtype).eps, atol=1e-4 * np.abs(gradient).max())
+
+
 # ---- calls that are allowed and unusual ---------------------------------------------------------------------------------
 @gpu
 def test_captured_backward_of_what_a_leaf_was_made_into():
@@ -851,13 +887,13 @@ def test_offsets_beyond_32_bits():
     assert torch.equal(got[-3:], ops.decay_attention_step(first, first, first, log_decay[:1], one)) and torch.equal(state[-3:], one)
     del state, x, got
     rows = (1 << 16) + 300
-    logits = normal(rows, 32768)
+    logits = normal(rows, 32768)                                   # (2 100 of them go the way of all)
     t = ops.top_logits(logits, 20)
-    end = ops.top_logits(logits[-300:].contiguous(), 20)
-    assert torch.equal(t.values[-300:], end.values) and torch.equal(t.indices[-300:], end.indices) and torch.equal(t.rest[-300:], end.rest)
+    end = ops.top_logits(logits[-2100:].contiguous(), 20)
+    assert torch.equal(t.values[-2100:], end.values) and torch.equal(t.indices[-2100:], end.indices) and torch.equal(t.rest[-2100:], end.rest)
     loss, grad = ops.distillation_loss_and_gradient(logits, ops.TopLogits(t.values * 2, t.indices, t.rest), None, 'none')
-    end = ops.distillation_loss_and_gradient(logits[-300:].contiguous(), ops.TopLogits(end.values * 2, end.indices, end.rest), None, 'none')
-    assert torch.equal(loss[-300:], end[0]) and torch.equal(grad[-300:], end[1])
+    end = ops.distillation_loss_and_gradient(logits[-2100:].contiguous(), ops.TopLogits(end.values * 2, end.indices, end.rest), None, 'none')
+    assert torch.equal(loss[-2100:], end[0]) and torch.equal(grad[-2100:], end[1])
 
 
 # ---- refusals (on the CPU: nothing is launched) -------------------------------------------------------------------------
