@@ -13,7 +13,7 @@
 // sixteen, by its length and the number of rows, and every lane reads 16 bytes at a time, four times before it computes.
 //   4 096 x 32 768 bf16, k = 32:      loss 75 us (3.6 TB/s), gradient 90 (6.0)
 //   1 023 x 131 071 f32, k = 100:     loss 108 to 147 (5.0 to 3.6), gradient 211 (5.1), where a copy of 2 GiB reaches 4.9
-//   2 047 x 50 001 bf16, k = 64:      the largest logits 72 (2.8): exponentials and comparisons fill the other half of the time
+//   2 047 x 50 001 bf16, k = 64:      the largest logits 62 (3.3): exponentials and comparisons fill half of the time
 //   10 000 x 5 f32 and 256 x 5 f32:   3.6, and 10 + 2 + 4.4: launches and the latency of a few dependent reductions
 #include "pxg_ops.h"
 #include <type_traits>
@@ -767,14 +767,19 @@ void launch_top(int64_t rows, int64_t classes, const void* logits, int64_t row_s
     if (classes <= 16) return narrow(std::integral_constant<int, 16>());
     if (classes <= 32) return narrow(std::integral_constant<int, 32>());
     if (classes <= 64) return narrow(std::integral_constant<int, 64>());
-    // a wave holds up to 32 (twice as many threads as are to be chosen), and serves many rows of up to 64 KB better than a workgroup
+    // A wave holds up to 32 (twice as many threads as are to be chosen), and serves many rows of up to 64 KB better than a workgroup
     // each (k = 4, four waves / one: 2 048 x 5 000 f32 22 / 14 us, 16 384 x 16 000 f16 159 / 110, 16 384 x 16 000 f32 201 / 188,
-    // 16 384 x 32 000 f32 354 / 364, 1 024 x 5 000 f16 12 / 11, 256 x 5 000 f32 11 / 11, 256 x 16 000 f32 14 / 19)
-    const bool one_wave = k <= 32 && (classes <= 1024 || (rows >= 2048 && classes * (int64_t)sizeof(T) <= 65536));
-    const int g = one_wave ? 64 : rows < 256 && classes > 16384 ? 1024 : 256;
+    // 16 384 x 32 000 f32 354 / 364, 1 024 x 5 000 f16 12 / 11, 256 x 5 000 f32 11 / 11, 256 x 16 000 f32 14 / 19).  Two waves hold
+    // up to 64, and are better than four in the same way (k = 64, four / two: 2 047 x 50 001 bf16 72 / 62, 2 047 x 50 001 f32
+    // 100 / 95, 16 384 x 2 000 f32 110 / 84, 16 384 x 8 000 f32 161 / 165, 16 384 x 20 000 f32 282 / 315, 512 x 20 000 bf16 19 / 24).
+    const bool short_rows = classes * (int64_t)sizeof(T) <= 65536;
+    const int g = k <= 32 && (classes <= 1024 || (rows >= 2048 && short_rows)) ? 64
+                : k <= 64 && rows >= 1024 && (short_rows || rows < 8192) ? 128
+                : rows < 256 && classes > 16384 ? 1024 : 256;
     const dim3 blocks = blocks_of(rows, g);
     switch (g) {
     case 64: k_top<64, T><<<blocks, 256, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest); break;
+    case 128: k_top<128, T><<<blocks, 128, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest); break;
     case 256: k_top<256, T><<<blocks, 256, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest); break;
     default: k_top<1024, T><<<blocks, 1024, 0, st>>>(rows, classes, (const T*)logits, row_stride, k, temperature, (T*)values, indices, rest);
     }

@@ -680,9 +680,10 @@ def test_captured_backward_beside_an_eager_graph():
 
 
 @gpu
-@pytest.mark.parametrize('rows,classes,k,dtype', [(2050, 5003, 31, 'f32'), (2048, 5001, 32, 'bf16'), (4097, 1031, 1, 'f16')])
+@pytest.mark.parametrize('rows,classes,k,dtype', [(2050, 5003, 31, 'f32'), (2048, 5001, 32, 'bf16'), (4097, 1031, 1, 'f16'),
+                                                  (1100, 3001, 64, 'f32'), (1030, 1200, 50, 'f16'), (1025, 33001, 20, 'bf16')])
 def test_top_logits_of_many_rows(rows, classes, k, dtype):
-    """a wave for each row, however long"""
+    """a wave or two for each row, however long"""
     inf, nan = math.inf, math.nan
     g = torch.Generator().manual_seed(classes)
     x = torch.randn(rows, classes, generator=g) * 3
