@@ -43,11 +43,9 @@ __device__ __forceinline__ float decay_over(float n, float log_a)
     return w > 0.f && w < INFINITY ? fmaf(w, lost, w) : w;
 }
 
-// steps in a chunk, by the type's number of bfloat16 planes and the padded width
-constexpr int decay_chunk(int dtype, int width)
-{
-    return 32;
-}
+constexpr int DECAY_CHUNK = 32;        // steps
+
+// the width that a head's are padded to
 constexpr int decay_width(int e, int f)
 {
     const int w = e > f ? e : f;

@@ -19,15 +19,15 @@ namespace {
 // writing the states: 128 pairs x 6 states of 64 x 64 6.5 us, three runs of them with slopes 12.4.
 constexpr int AT_ONCE = 8;
 
-__global__ __launch_bounds__(256) void k_decay_join(const DecayRuns a, int chunk, int slope_runs)
+__global__ __launch_bounds__(256) void k_decay_join(const DecayRuns a, int slope_runs)
 {
     const DecayRun& r = a.run[blockIdx.z];
     const int64_t size = (int64_t)r.E * r.F, bh = blockIdx.x, n = a.segments - 1;
     const int64_t slopes = (int64_t)a.batch * a.heads * n * size;
     const int i = blockIdx.y * 256 + threadIdx.x;
     if (i >= size) return;
-    const int used = (int)((uint32_t)(decay_length(a, (int)bh / a.heads) + chunk - 1) / (uint32_t)chunk);
-    const float steps = (float)a.segment_chunks * (float)chunk, decay = decay_over(steps, a.log_decay[(int)bh % a.heads]);
+    const int used = (int)((uint32_t)(decay_length(a, (int)bh / a.heads) + DECAY_CHUNK - 1) / DECAY_CHUNK);
+    const float steps = (float)a.segment_chunks * (float)DECAY_CHUNK, decay = decay_over(steps, a.log_decay[(int)bh % a.heads]);
     const bool slope = (int)blockIdx.z < slope_runs;
     float* c = r.carry + bh * n * size + i;
     float S = c[0], G = slope ? c[slopes] : 0.f;
@@ -82,7 +82,7 @@ int launch_runs(const DecayRuns& a, int dtype, int n, int slopes, hipStream_t st
         const int rc = launch(a, dtype, n, slopes, true, stream);
         if (rc != PXG_OK) return rc;
         const dim3 grid(a.batch * a.heads, (a.run[0].E * a.run[0].F + 255) / 256, n);
-        k_decay_join<<<grid, 256, 0, stream>>>(a, decay_chunk(dtype, decay_width(a.run[0].E, a.run[0].F)), slopes);
+        k_decay_join<<<grid, 256, 0, stream>>>(a, slopes);
         if (hipGetLastError() != hipSuccess) return PXG_E_HIP;
     }
     return launch(a, dtype, n, slopes, false, stream);
@@ -208,7 +208,7 @@ struct Cut {
 Cut cut_of(const pxg_decay* a, bool backward)
 {
     const int width = decay_width(a->dk, a->dv);
-    const int64_t chunk = decay_chunk(a->dtype, width), chunks = (a->steps + chunk - 1) / chunk;
+    const int64_t chunks = (a->steps + DECAY_CHUNK - 1) / DECAY_CHUNK;
     const int64_t waves = a->batch * a->heads * (width / 16);
     int64_t segments = 1;
     if (waves > 0 && waves <= (backward ? 1023 : 1024)) segments = ((backward ? 2048 : 4096) + waves - 1) / waves;

@@ -213,7 +213,7 @@ constexpr int waves_wanted(int planes, int width, bool slope, bool states_only)
 
 // Shared memory of one workgroup, as separate arrays: what is written to one does not hold up what is read from another.
 #define DECAY_SHARED(T, D, SLOPE, STATES_ONLY)                                                                                          \
-    constexpr int SETS = STATES_ONLY ? 2 : SLOPE ? 4 : 3, CHUNK = decay_chunk(Type<T>::code, D);                                      \
+    constexpr int SETS = STATES_ONLY ? 2 : SLOPE ? 4 : 3, CHUNK = DECAY_CHUNK;                                     \
     constexpr int WEIGHT_PLANES = STATES_ONLY || D == 16 ? 0 : Type<T>::planes == 3 ? 3 : 2;                                          \
     __shared__ __attribute__((aligned(16))) __bf16 tile[SETS * Type<T>::planes * CHUNK * Shape<D>::row];                              \
     __shared__ __attribute__((aligned(16))) __bf16 weights[WEIGHT_PLANES ? WEIGHT_PLANES * CHUNK * (CHUNK + 8) : 8];                  \
@@ -226,7 +226,7 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
                                             float* const pw, double* const sums, int* const strange)
 {
     using Sh = Shape<D>;
-    constexpr int NP = Type<T>::planes, C = decay_chunk(Type<T>::code, D), CT = C / 16, ET = Sh::et, KB = Sh::kb;
+    constexpr int NP = Type<T>::planes, C = DECAY_CHUNK, CT = C / 16, ET = Sh::et, KB = Sh::kb;
     constexpr int ROW = Sh::row, PLANE = C * ROW, N = Sh::threads, W = Sh::waves, PIECES = C * (D / 8) / N;
     constexpr int KEEP = NP == 3 ? 2 : 1;                     // products of planes p + q <= KEEP go into the result
     constexpr int PROW = C + 8, PPLANE = C * PROW;            // of the weights
@@ -429,15 +429,13 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
             for (int turn = 0; turn < (TILES + W - 1) / W; turn++) {
                 const int n = W == 1 ? turn : wave + turn * W;
                 if (n >= TILES) break;
-                const int it = n < 1 ? 0 : n < 3 ? 1 : n < 6 ? 2 : 3, jt = n - it * (it + 1) / 2;
+                const int it = n < 1 ? 0 : 1, jt = n - it;               // two tiles of 16: (0, 0), (1, 0), (1, 1)
                 f32x4 acc = products(ty, tx, jt, it);
                 if (it == jt) {
 #pragma unroll
                     for (int s = 0; s < 4; s++) acc[s] = li >= 4 * g + s ? acc[s] * w_diag[s] : 0.f;
                 } else {
                     acc *= w_off;
-                    if (it - jt == 2) acc *= tiles[1];
-                    if (CT > 2 && it - jt == 3) acc *= tiles[CT > 2 ? 2 : 0];
                 }
                 bf16x4 u[KEEP + 1];
                 split<KEEP + 1>(acc, u);
