@@ -259,7 +259,9 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
     }
 
     const float log_a = a.log_decay[h];
-    for (int n = tid; n <= C; n += N) pw[n] = n ? decay_over((float)n, log_a) : 1.f;
+    // More steps than the sequence has lie between no two of its rows, only between the empty ones in front (whose zeros a decay
+    // that grows out of float32 would turn into NaN: one step, log_decay = 3): 0 for those.
+    for (int n = tid; n <= C; n += N) pw[n] = n == 0 ? 1.f : n <= len ? decay_over((float)n, log_a) : 0.f;
     if (tid < 2) strange[tid] = 0;
     __syncthreads();
     // factors of one lane: inside a diagonal tile, for tiles further off, for the state (index: step 4 g + s of a tile)

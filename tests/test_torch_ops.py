@@ -278,6 +278,27 @@ def test_decay_attention_extreme_decays():
 
 
 @gpu
+@pytest.mark.parametrize('dtype', sorted(TYPES))
+@pytest.mark.parametrize('state', [False, True])
+@pytest.mark.parametrize('steps', [1, 2, 17, 30, 33, 70, 700])
+def test_decay_attention_growing_decays(steps, state, dtype):
+    """log_decay above 0: numbers as long as exp(log_decay * steps) is one, however short the sequences are"""
+    p = problem(5, steps, 3, 16, 24, dtype, True, state, seed=40)
+    # (the gradient of log_decay is `steps` times a sum of such factors; float16 results end at 65 504, without a state and with
+    # one step they do not depend on the decay)
+    most = 3.0 if dtype == 'f16' and (state or steps > 1) else 60.0
+    p['log_decay'] = torch.tensor([most / steps, 0.5 / steps, -0.1])
+    d = to_gpu(p)
+    got = ops.decay_attention(**{x: d[x] for x in ARGS}, return_state=True)
+    want = recurrence(*[to_f64(p)[x] for x in ARGS])
+    size = recurrence(*[to_f64(absolute(p))[x] for x in ARGS])
+    for x, y, z in zip(got, want, size):
+        assert_near(x, y, z, steps)
+    grads = ops.decay_attention_backward(d['grad_out'], *[d[x] for x in ARGS], grad_state=d['grad_state'])
+    check_gradients({x: y for x, y in zip(LEAVES, grads) if y is not None}, p, (5, steps, 3, 16, 24))
+
+
+@gpu
 def test_decay_attention_empty_and_long():
     for b, t in ((0, 5), (2, 0)):
         p = to_gpu(problem(max(b, 1), max(t, 1), 2, 8, 8, 'f32', state=True))
