@@ -182,10 +182,14 @@ class TopLogits:
 
     @staticmethod
     def cat(parts):
+        """All rows of several answers of one temperature.  Where only some of them have a rest, the others get one of nothing
+        (-inf: their listed classes are all there is)."""
         parts = list(parts)
-        rest = None if any(p.rest is None for p in parts) else torch.cat([p.rest for p in parts])
         if len({p.temperature for p in parts}) != 1:
             raise ValueError('answers of different temperatures')
+        rest = None
+        if any(p.rest is not None for p in parts):
+            rest = torch.cat([torch.full((len(p),), float('-inf'), device=p.values.device) if p.rest is None else p.rest for p in parts])
         return TopLogits(torch.cat([p.values for p in parts]), torch.cat([p.indices for p in parts]), rest, parts[0].temperature)
 
 

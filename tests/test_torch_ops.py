@@ -1008,6 +1008,31 @@ def test_top_logits_rows():
     assert ops.TopLogits(t.values, t.indices)[0].rest is None
 
 
+def mixed_parts():
+    x, t, weight = distill_problem(6, 40, 3, 'f32', 2.0, seed=41)
+    return x, weight, [t[:2], ops.TopLogits(t.values[2:5], t.indices[2:5], None, 2.0), t[5:]], t
+
+
+def test_answers_with_and_without_a_rest_are_joined():
+    x, weight, parts, t = mixed_parts()
+    for order in ([0, 1, 2], [1, 0, 2], [1, 2]):
+        both = ops.TopLogits.cat([parts[i] for i in order])
+        want = torch.cat([torch.full((3,), -math.inf) if i == 1 else parts[i].rest for i in order])
+        assert both.rest.equal(want) and both.rest.dtype == torch.float32 and both.values.equal(torch.cat([parts[i].values for i in order]))
+    assert ops.TopLogits.cat([parts[1], parts[1]]).rest is None
+    assert ops.TopLogits.cat([t[:0], parts[1]]).rest.equal(torch.full((3,), -math.inf))
+
+
+@gpu
+def test_joined_answers_have_the_losses_of_their_parts():
+    x, weight, parts, _ = mixed_parts()
+    x, weight, parts = x.cuda(), weight.cuda(), [p.to('cuda') for p in parts]
+    loss, grad = ops.distillation_loss_and_gradient(x, ops.TopLogits.cat(parts), weight, 'none')
+    rows = torch.arange(6).split([2, 3, 1])
+    alone = [ops.distillation_loss_and_gradient(x[r], p, weight[r], 'none') for r, p in zip(rows, parts)]
+    assert torch.equal(loss, torch.cat([a for a, _ in alone])) and torch.equal(grad, torch.cat([b for _, b in alone]))
+
+
 def test_c_entries_refuse_what_they_can_see():
     """bad shapes, types and missing pointers come back as PXG_E_INVALID before anything touches a GPU"""
     lib = N.load_library()
