@@ -185,6 +185,8 @@ class TopLogits:
         """All rows of several answers of one temperature.  Where only some of them have a rest, the others get one of nothing
         (-inf: their listed classes are all there is)."""
         parts = list(parts)
+        if not parts:
+            raise ValueError('no answers to join')
         if len({p.temperature for p in parts}) != 1:
             raise ValueError('answers of different temperatures')
         rest = None

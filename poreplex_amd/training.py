@@ -176,6 +176,8 @@ def distillation_targets(teacher, x, k=3, temperature=2.0, device='cuda', batch_
     """The teacher's `k` largest answers to every sample of x (torch_ops.TopLogits on the CPU): the targets of
     ``Trainer(model, torch_ops.distillation_loss).fit(x, targets)``."""
     from . import torch_ops
+    if len(x) == 0:
+        raise ValueError('no samples to ask the teacher about')
     device, parts = torch.device(device), []
     teacher = teacher.to(device).eval()
     with torch.no_grad():

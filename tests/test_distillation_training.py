@@ -36,6 +36,13 @@ def test_refusals(tmp_path):
         TR.DemuxClassifier(top='decay')(torch.zeros(2, 300))
 
 
+def test_no_samples_and_no_answers_are_refused():
+    with pytest.raises(ValueError, match='no samples'):
+        TR.distillation_targets(TR.DemuxClassifier(), torch.zeros(0, 300), device='cpu')
+    with pytest.raises(ValueError, match='no answers'):
+        ops.TopLogits.cat([])
+
+
 def test_trainer_takes_top_logits(tmp_path):
     """Targets that are TopLogits go through the trainer's split, shuffling and batches like labels: every sample meets its own."""
     n = 70
