@@ -101,6 +101,14 @@ void refuse_captured_leaves(std::initializer_list<const Tensor*> tensors, const 
     }
 }
 
+// The autograd nodes here have no forward mode, and where no gradient is wanted there is no node at all to say so: a dual tensor's
+// tangent would be dropped without a word.
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors)
+{
+    for (const Tensor* t : tensors)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
 bool wants_graph(std::initializer_list<const Tensor*> tensors)
 {
     if (!at::GradMode::is_enabled()) return false;
@@ -215,6 +223,7 @@ std::pair<Tensor, MaybeTensor> decay_attention(const Tensor& q, const Tensor& k,
                                                const MaybeTensor& lengths, const MaybeTensor& initial, bool want_state)
 {
     const Tensor start = initial.value_or(Tensor());
+    refuse_tangents("decay_attention", {&q, &k, &v, &log_decay, &start});
     Tensor out, state;
     if (wants_graph({&q, &k, &v, &log_decay, &start})) {
         refuse_captured_leaves({&q, &k, &v, &log_decay, &start}, q);
@@ -231,6 +240,8 @@ py::tuple decay_attention_backward(const Tensor& grad_out, const Tensor& q, cons
                                    const MaybeTensor& lengths, const MaybeTensor& initial, const MaybeTensor& grad_state)
 {
     at::NoGradGuard no_grad;
+    const Tensor start = initial.value_or(Tensor()), end = grad_state.value_or(Tensor());
+    refuse_tangents("decay_attention_backward", {&grad_out, &q, &k, &v, &log_decay, &start, &end});
     const auto g = decay_backward(grad_out, q, k, v, log_decay, lengths, initial, grad_state, true, initial.has_value());
     return py::make_tuple(g.q, g.k, g.v, g.log_decay, initial ? py::cast(g.initial) : py::object(py::none()));
 }
@@ -238,6 +249,7 @@ py::tuple decay_attention_backward(const Tensor& grad_out, const Tensor& q, cons
 Tensor decay_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state, const MaybeTensor& active_)
 {
     at::NoGradGuard no_grad;
+    refuse_tangents("decay_attention_step", {&q, &k, &v, &log_decay, &state});
     const c10::DeviceGuard device(q.device());
     DecayCall c(q, k, v, log_decay, std::nullopt, std::nullopt);
     const Tensor active = contiguous(active_), out = empty(v.sizes(), v, v.scalar_type());
@@ -333,6 +345,8 @@ struct Distillation : torch::autograd::Function<Distillation> {
 Tensor distillation_loss(const Tensor& logits, const Tensor& values, const Tensor& indices, const MaybeTensor& rest,
                          const MaybeTensor& weight, double temperature, int reduction)
 {
+    const Tensor r = rest.value_or(Tensor()), w = weight.value_or(Tensor());
+    refuse_tangents("distillation_loss", {&logits, &values, &r, &w});
     if (!wants_graph({&logits})) return distill_forward(logits, values, indices, rest, weight, temperature, reduction).first;
     refuse_captured_leaves({&logits}, logits);
     return Distillation::apply(logits, values, indices, rest, weight, temperature, (int64_t)reduction);
@@ -343,6 +357,8 @@ std::pair<Tensor, Tensor> distillation_loss_and_gradient(const Tensor& logits, c
                                                          int reduction, const MaybeTensor& grad_loss)
 {
     at::NoGradGuard no_grad;
+    const Tensor r = rest.value_or(Tensor()), w = weight.value_or(Tensor()), from = grad_loss.value_or(Tensor());
+    refuse_tangents("distillation_loss_and_gradient", {&logits, &values, &r, &w, &from});
     auto [loss, held] = distill_forward(logits, values, indices, rest, weight, temperature, reduction);
     const Tensor scale = grad_loss ? *grad_loss : at::ones(loss.sizes(), loss.options());
     return {loss, distill_backward(scale, logits, values, indices, weight, held, temperature, reduction)};

@@ -9,7 +9,8 @@ csrc/k_distill.hip behind include/pxg.h).
                          teach others (``training.Trainer`` takes it as its ``loss_fn``)
 
 Tensors live on one GPU; calls run on the current stream of that GPU and return without waiting.  They only launch kernels, so
-they may be captured into a graph.  The library missing or a tensor on another device raises: there is no fallback.
+they may be captured into a graph.  The library missing or a tensor on another device raises: there is no fallback.  Derivatives are
+those of one backward pass: a second one and forward-mode tangents raise NotImplementedError.
 
 Arguments are checked here; csrc/pxg_torch.cpp makes the calls and is the autograd node.
 """

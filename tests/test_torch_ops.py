@@ -1008,6 +1008,63 @@ def test_top_logits_rows():
     assert ops.TopLogits(t.values, t.indices)[0].rest is None
 
 
+@pytest.fixture
+def idle(monkeypatch):
+    """the extension over entry points that do nothing but fail: CPU tensors pass as GPU tensors, nothing is ever launched"""
+    monkeypatch.setattr(ops, '_on_gpu', lambda name, t, device=None: None)
+    ext, lib = ops._ext(), N.load_library()
+    fails = C.CFUNCTYPE(C.c_int64)(lambda: -1)
+    ext.use_library([C.cast(fails, C.c_void_p).value] * len(ops._ENTRY_POINTS))
+    yield
+    ext.use_library([C.cast(getattr(lib, name), C.c_void_p).value for name in ops._ENTRY_POINTS])
+
+
+def every_call(p, change=lambda name, t: t):
+    """(name, call) of every public call, with `change` made to one tensor at a time"""
+    x, teacher, weight = distill_problem(3, 9, 2, 'f32', 2.0, seed=43)
+    step = {n: p[n][:, 0] for n in 'qkv'}
+    for n in ARGS + ('grad_out', 'grad_state'):
+        if p[n].is_floating_point():
+            if n in ARGS:
+                yield 'decay_attention', lambda: ops.decay_attention(**{m: change(m, p[m]) if m == n else p[m] for m in ARGS})
+                if n in step or n == 'log_decay':
+                    yield 'decay_attention_step', lambda: ops.decay_attention_step(**{**step, 'log_decay': p['log_decay'], n: change(
+                        n, step.get(n, p['log_decay']))}, state=p['initial_state'])
+            yield 'decay_attention_backward', lambda: ops.decay_attention_backward(**{m: change(m, p[m]) if m == n else p[m] for m in ARGS + (
+                'grad_out', 'grad_state')})
+    yield 'decay_attention_step', lambda: ops.decay_attention_step(**step, log_decay=p['log_decay'], state=change('state', p['initial_state']))
+    dev = p['q'].device
+    call = {'logits': x.to(dev), 'values': teacher.values.to(dev), 'rest': teacher.rest.to(dev), 'weight': weight.to(dev)}
+    for n in call:
+        for name in ('distillation_loss', 'distillation_loss_and_gradient'):
+            def one():
+                c = {**call, n: change(n, call[n])}
+                return getattr(ops, name)(c['logits'], ops.TopLogits(c['values'], teacher.indices.to(dev), c['rest'], 2.0), c['weight'])
+            yield name, one
+
+
+def tangents_are_refused(p):
+    fw, seen = torch.autograd.forward_ad, set()
+    with fw.dual_level():
+        for name, call in every_call(p, lambda n, t: fw.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(NotImplementedError, match=name + ' has no forward-mode derivative'):
+                call()
+            seen.add(name)
+    assert len(seen) == 5
+
+
+def test_tangents_are_refused(idle):
+    tangents_are_refused(problem(2, 4, 1, 8, 8, 'f32', True, True, seed=42))
+
+
+@gpu
+def test_tangents_are_refused_on_the_gpu():
+    p = to_gpu(problem(2, 4, 1, 8, 8, 'f32', True, True, seed=42))
+    tangents_are_refused(p)
+    with torch.autograd.forward_ad.dual_level():                    # numbers without a tangent are no matter of it
+        assert torch.isfinite(ops.decay_attention(**{n: p[n] for n in ARGS})).all()
+
+
 def mixed_parts():
     x, t, weight = distill_problem(6, 40, 3, 'f32', 2.0, seed=41)
     return x, weight, [t[:2], ops.TopLogits(t.values[2:5], t.indices[2:5], None, 2.0), t[5:]], t
