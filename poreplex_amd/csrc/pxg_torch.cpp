@@ -5,10 +5,12 @@
 // tensor), launches on the current stream of the tensors' device, and the autograd nodes run without the interpreter.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 #include <unordered_set>
 #include "../../include/pxg.h"
@@ -107,6 +109,14 @@ void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tens
 {
     for (const Tensor* t : tensors)
         TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative");
+}
+
+// A recording of torch's own calls holds nothing of what the kernels write: its result would be an empty tensor.
+void refuse_recording(const char* what)
+{
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() &&
+                                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+                                what, " cannot be traced (torch.jit.trace, make_fx): a recording does not see its kernels");
 }
 
 bool wants_graph(std::initializer_list<const Tensor*> tensors)
@@ -223,6 +233,7 @@ std::pair<Tensor, MaybeTensor> decay_attention(const Tensor& q, const Tensor& k,
                                                const MaybeTensor& lengths, const MaybeTensor& initial, bool want_state)
 {
     const Tensor start = initial.value_or(Tensor());
+    refuse_recording("decay_attention");
     refuse_tangents("decay_attention", {&q, &k, &v, &log_decay, &start});
     Tensor out, state;
     if (wants_graph({&q, &k, &v, &log_decay, &start})) {
@@ -241,6 +252,7 @@ py::tuple decay_attention_backward(const Tensor& grad_out, const Tensor& q, cons
 {
     at::NoGradGuard no_grad;
     const Tensor start = initial.value_or(Tensor()), end = grad_state.value_or(Tensor());
+    refuse_recording("decay_attention_backward");
     refuse_tangents("decay_attention_backward", {&grad_out, &q, &k, &v, &log_decay, &start, &end});
     const auto g = decay_backward(grad_out, q, k, v, log_decay, lengths, initial, grad_state, true, initial.has_value());
     return py::make_tuple(g.q, g.k, g.v, g.log_decay, initial ? py::cast(g.initial) : py::object(py::none()));
@@ -249,6 +261,7 @@ py::tuple decay_attention_backward(const Tensor& grad_out, const Tensor& q, cons
 Tensor decay_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, const Tensor& state, const MaybeTensor& active_)
 {
     at::NoGradGuard no_grad;
+    refuse_recording("decay_attention_step");
     refuse_tangents("decay_attention_step", {&q, &k, &v, &log_decay, &state});
     const c10::DeviceGuard device(q.device());
     DecayCall c(q, k, v, log_decay, std::nullopt, std::nullopt);
@@ -263,6 +276,7 @@ Tensor decay_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
 std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& logits_, int64_t k, double temperature)
 {
     at::NoGradGuard no_grad;
+    refuse_recording("top_logits");
     const c10::DeviceGuard device(logits_.device());
     const Tensor logits = rows(logits_);
     const int64_t n = logits.size(0);
@@ -346,6 +360,7 @@ Tensor distillation_loss(const Tensor& logits, const Tensor& values, const Tenso
                          const MaybeTensor& weight, double temperature, int reduction)
 {
     const Tensor r = rest.value_or(Tensor()), w = weight.value_or(Tensor());
+    refuse_recording("distillation_loss");
     refuse_tangents("distillation_loss", {&logits, &values, &r, &w});
     if (!wants_graph({&logits})) return distill_forward(logits, values, indices, rest, weight, temperature, reduction).first;
     refuse_captured_leaves({&logits}, logits);
@@ -358,6 +373,7 @@ std::pair<Tensor, Tensor> distillation_loss_and_gradient(const Tensor& logits, c
 {
     at::NoGradGuard no_grad;
     const Tensor r = rest.value_or(Tensor()), w = weight.value_or(Tensor()), from = grad_loss.value_or(Tensor());
+    refuse_recording("distillation_loss_and_gradient");
     refuse_tangents("distillation_loss_and_gradient", {&logits, &values, &r, &w, &from});
     auto [loss, held] = distill_forward(logits, values, indices, rest, weight, temperature, reduction);
     const Tensor scale = grad_loss ? *grad_loss : at::ones(loss.sizes(), loss.options());

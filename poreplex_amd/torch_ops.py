@@ -10,7 +10,8 @@ csrc/k_distill.hip behind include/pxg.h).
 
 Tensors live on one GPU; calls run on the current stream of that GPU and return without waiting.  They only launch kernels, so
 they may be captured into a graph.  The library missing or a tensor on another device raises: there is no fallback.  Derivatives are
-those of one backward pass: a second one and forward-mode tangents raise NotImplementedError.
+those of one backward pass: a second one and forward-mode tangents raise NotImplementedError, and so does a call that is being
+recorded (torch.jit.trace, make_fx): torch sees nothing of these kernels.
 
 Arguments are checked here; csrc/pxg_torch.cpp makes the calls and is the autograd node.
 """

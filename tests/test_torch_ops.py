@@ -1026,18 +1026,18 @@ def every_call(p, change=lambda name, t: t):
     for n in ARGS + ('grad_out', 'grad_state'):
         if p[n].is_floating_point():
             if n in ARGS:
-                yield 'decay_attention', lambda: ops.decay_attention(**{m: change(m, p[m]) if m == n else p[m] for m in ARGS})
+                yield 'decay_attention', lambda n=n: ops.decay_attention(**{m: change(m, p[m]) if m == n else p[m] for m in ARGS})
                 if n in step or n == 'log_decay':
-                    yield 'decay_attention_step', lambda: ops.decay_attention_step(**{**step, 'log_decay': p['log_decay'], n: change(
+                    yield 'decay_attention_step', lambda n=n: ops.decay_attention_step(**{**step, 'log_decay': p['log_decay'], n: change(
                         n, step.get(n, p['log_decay']))}, state=p['initial_state'])
-            yield 'decay_attention_backward', lambda: ops.decay_attention_backward(**{m: change(m, p[m]) if m == n else p[m] for m in ARGS + (
+            yield 'decay_attention_backward', lambda n=n: ops.decay_attention_backward(**{m: change(m, p[m]) if m == n else p[m] for m in ARGS + (
                 'grad_out', 'grad_state')})
     yield 'decay_attention_step', lambda: ops.decay_attention_step(**step, log_decay=p['log_decay'], state=change('state', p['initial_state']))
     dev = p['q'].device
     call = {'logits': x.to(dev), 'values': teacher.values.to(dev), 'rest': teacher.rest.to(dev), 'weight': weight.to(dev)}
     for n in call:
         for name in ('distillation_loss', 'distillation_loss_and_gradient'):
-            def one():
+            def one(name=name, n=n):
                 c = {**call, n: change(n, call[n])}
                 return getattr(ops, name)(c['logits'], ops.TopLogits(c['values'], teacher.indices.to(dev), c['rest'], 2.0), c['weight'])
             yield name, one
@@ -1063,6 +1063,38 @@ def test_tangents_are_refused_on_the_gpu():
     tangents_are_refused(p)
     with torch.autograd.forward_ad.dual_level():                    # numbers without a tangent are no matter of it
         assert torch.isfinite(ops.decay_attention(**{n: p[n] for n in ARGS})).all()
+
+
+def recordings_are_refused(p):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    calls, seen = list(every_call(p)), set()
+    calls.append(('top_logits', lambda: ops.top_logits(p['q'][:, 0, 0], 3).values))
+    for name, call in calls:
+        if name in seen:
+            continue
+        seen.add(name)
+        with pytest.raises(NotImplementedError, match=name + ' cannot be traced'):
+            torch.jit.trace(lambda x: (call(), x)[1], p['q'], check_trace=False)
+        with pytest.raises(NotImplementedError, match=name + ' cannot be traced'):
+            make_fx(lambda x: (call(), x)[1])(p['q'])
+    assert len(seen) == 6
+
+
+@pytest.mark.filterwarnings('ignore::torch.jit.TracerWarning')
+def test_recordings_are_refused(idle):
+    recordings_are_refused(problem(2, 4, 1, 8, 8, 'f32', True, True, seed=44))
+
+
+@gpu
+@pytest.mark.filterwarnings('ignore::torch.jit.TracerWarning')
+def test_recordings_are_refused_on_the_gpu():
+    p = to_gpu(problem(2, 4, 1, 8, 8, 'f32', True, True, seed=44))
+    recordings_are_refused(p)
+    assert torch.isfinite(ops.decay_attention(**{n: p[n] for n in ARGS})).all()
+    # what breaks a graph at such a call instead of recording through it goes on as it did
+    want = ops.decay_attention(**{n: p[n] for n in ARGS}) * 2
+    got = torch.compile(lambda q: ops.decay_attention(**{**{n: p[n] for n in ARGS}, 'q': q}) * 2, backend='eager')(p['q'])
+    assert torch.equal(got, want)
 
 
 def mixed_parts():
