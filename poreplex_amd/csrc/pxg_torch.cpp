@@ -267,8 +267,8 @@ Tensor decay_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
     DecayCall c(q, k, v, log_decay, std::nullopt, std::nullopt);
     const Tensor active = contiguous(active_), out = empty(v.sizes(), v, v.scalar_type());
     c.s.lengths = data<void>(active), c.s.out = out.data_ptr(), c.s.final_state = data<float>(state);
+    state.unsafeGetTensorImpl()->bump_version();      // written in place; first, for this is what refuses a state of inference mode
     check("pxg_decay_step", lib.decay_step(&c.s, stream_of(q)));
-    state.unsafeGetTensorImpl()->bump_version();      // written in place
     return out;
 }
 

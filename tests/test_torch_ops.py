@@ -1065,6 +1065,24 @@ def test_tangents_are_refused_on_the_gpu():
         assert torch.isfinite(ops.decay_attention(**{n: p[n] for n in ARGS})).all()
 
 
+def refused_state(p):
+    with torch.inference_mode():
+        state = p['initial_state'].clone()
+    with pytest.raises(RuntimeError, match='[Ii]nference'):
+        ops.decay_attention_step(*[p[n][:, 0] for n in 'qkv'], p['log_decay'], state)
+    return state
+
+
+def test_a_state_of_inference_mode_is_refused_outside_it(idle):
+    refused_state(problem(2, 4, 1, 8, 8, 'f32', True, True, seed=45))      # (had it been launched, another error)
+
+
+@gpu
+def test_a_refused_state_is_left_as_it_was():
+    p = to_gpu(problem(2, 4, 1, 8, 8, 'f32', True, True, seed=45))
+    assert torch.equal(refused_state(p), p['initial_state'])
+
+
 def recordings_are_refused(p):
     from torch.fx.experimental.proxy_tensor import make_fx
     calls, seen = list(every_call(p)), set()
