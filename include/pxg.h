@@ -710,7 +710,8 @@ int pxg_decay_backward(const pxg_decay* call, void* stream);
 int pxg_decay_step(const pxg_decay* call, void* stream);
 
 /* The k largest of each row's `classes` logits in descending order (ties: lowest class first; NaN counts as the largest),
- * their classes, and rest[row] = log sum over the OTHER classes of exp(logit / temperature) (-inf where there is none). */
+ * their classes, and rest[row] = log sum over the OTHER classes of exp(logit / temperature) (-inf where there is none).
+ * A temperature, here and below, is a normal number of up to 3e38. */
 int pxg_top_logits(int32_t dtype, int64_t rows, int64_t classes, const void* logits, int64_t row_stride, int32_t k,
                    float temperature, void* values, int32_t* indices, float* rest, void* stream);
 

@@ -815,12 +815,15 @@ template <typename T> void launch_backward(const pxg_distill& a, hipStream_t st)
     }
 }
 
+// below the least normal number its reciprocal is no float32 (scale_of): 0 times that would be NaN
+bool bad_temperature(float t) { return !(t >= 1.17549435e-38f && t <= 3.0e38f); }
+
 bool bad_call(const pxg_distill* a)
 {
     return !a || a->struct_bytes != sizeof(pxg_distill) || a->dtype < PXG_DT_F32 || a->dtype > PXG_DT_F16 ||
            a->value_dtype < PXG_DT_F32 || a->value_dtype > PXG_DT_F16 || a->rows < 0 || a->rows > INT32_MAX || a->classes < 1 ||
-           a->classes > INT32_MAX || a->k < 0 || a->k > PXG_TOP_MAX_K || !(a->temperature > 0.f) ||
-           a->temperature > 3.0e38f || (a->rows > 0 && (!a->logits || !a->stats || (a->k > 0 && (!a->values || !a->indices))));
+           a->classes > INT32_MAX || a->k < 0 || a->k > PXG_TOP_MAX_K || bad_temperature(a->temperature) ||
+           (a->rows > 0 && (!a->logits || !a->stats || (a->k > 0 && (!a->values || !a->indices))));
 }
 
 }  // namespace
@@ -829,7 +832,7 @@ extern "C" int pxg_top_logits(int32_t dtype, int64_t rows, int64_t classes, cons
                               float temperature, void* values, int32_t* indices, float* rest, void* stream)
 {
     if (dtype < PXG_DT_F32 || dtype > PXG_DT_F16 || rows < 0 || rows > INT32_MAX || classes < 1 || classes > INT32_MAX || k < 1 ||
-        k > PXG_TOP_MAX_K || k > classes || !(temperature > 0.f) || temperature > 3.0e38f)
+        k > PXG_TOP_MAX_K || k > classes || bad_temperature(temperature))
         return PXG_E_INVALID;
     if (rows == 0) return PXG_OK;
     if (!logits || !values || !indices || !rest) return PXG_E_INVALID;

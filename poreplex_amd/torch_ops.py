@@ -199,8 +199,8 @@ class TopLogits:
 
 def _temperature(temperature):
     temperature = float(temperature)
-    if not 0.0 < temperature <= 3.0e38:
-        raise ValueError('temperature is {}: a positive number is needed'.format(temperature))
+    if not 1.2e-38 <= temperature <= 3.0e38:                       # and what float32 holds as a normal number
+        raise ValueError('temperature is {}: a positive number of 1.2e-38 to 3e38 is needed'.format(temperature))
     return temperature
 
 

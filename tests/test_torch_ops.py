@@ -1065,6 +1065,22 @@ def test_tangents_are_refused_on_the_gpu():
         assert torch.isfinite(ops.decay_attention(**{n: p[n] for n in ARGS})).all()
 
 
+def test_temperatures_below_the_least_normal_number_are_refused(dry):
+    lib = N.load_library()
+    d = N.PxgDistill()
+    d.struct_bytes, d.rows, d.classes, d.k = C.sizeof(d), 0, 8, 0
+    for tau in (1e-39, 1e-50, 1.1e-38, -1.0, 3.1e38):
+        with pytest.raises(ValueError, match='temperature'):
+            ops.top_logits(torch.zeros(2, 3), 1, tau)
+        with pytest.raises(ValueError, match='temperature'):
+            ops.distillation_loss(torch.zeros(2, 3), ops.TopLogits(torch.zeros(2, 1), torch.zeros(2, 1).int(), None, tau))
+        d.temperature = tau
+        assert lib.pxg_distill_forward(C.byref(d), None) == -1 and lib.pxg_top_logits(0, 0, 8, None, 8, 2, tau, None, None, None, None) == -1
+    for tau in (1.2e-38, 1.0, 3e38):
+        d.temperature = tau
+        assert lib.pxg_distill_forward(C.byref(d), None) == 0 and lib.pxg_top_logits(0, 0, 8, None, 8, 2, tau, None, None, None, None) == 0
+
+
 def refused_state(p):
     with torch.inference_mode():
         state = p['initial_state'].clone()
