@@ -86,7 +86,7 @@ template <typename T> __device__ __forceinline__ Scale scale_of(float temperatur
     Scale s = {(float)c, 0.f};
     if (sizeof(T) == 4) {
         if ((double)s.hi >= c) s.hi = __uint_as_float(__float_as_uint(s.hi) - 1);
-        s.lo = (float)(c - (double)s.hi);
+        s.lo = fmaxf((float)(c - (double)s.hi), 0x1p-149f);       // (0 from temperatures of 1e29 or so on)
     }
     return s;
 }

@@ -1081,6 +1081,21 @@ def test_temperatures_below_the_least_normal_number_are_refused(dry):
         assert lib.pxg_distill_forward(C.byref(d), None) == 0 and lib.pxg_top_logits(0, 0, 8, None, 8, 2, tau, None, None, None, None) == 0
 
 
+@gpu
+def test_extreme_temperatures():
+    for classes in (9, 300):
+        x = torch.zeros(2, classes)
+        x[:, 0], x[1, 1:] = 1.0, torch.linspace(-1.0, 0.0, classes - 1)
+        for tau in (1.2e-38, 3e38):
+            t = ops.top_logits(x.cuda(), 1, tau)
+            # equal ones: their number; else the largest counts alone, or all do
+            want = [math.log(classes - 1), 0.0 if tau < 1 else math.log(classes - 1)]
+            assert t.indices[:, 0].tolist() == [0, 0] and np.allclose(t.rest.cpu().numpy(), want, atol=1e-6)
+            # the listed class far ahead of all others, or as good as each of them
+            loss, grad = ops.distillation_loss_and_gradient(x.cuda(), t, reduction='none')
+            assert torch.isfinite(grad).all() and float(loss.abs().max()) <= (1e-30 if tau < 1 else math.inf)
+
+
 def refused_state(p):
     with torch.inference_mode():
         state = p['initial_state'].clone()
