@@ -179,14 +179,18 @@ template <int G, typename T, typename F> __device__ __forceinline__ void each_un
 // goes by, at the first tiles of 4 units a thread and then ever more rarely.  A unit below the bound is added to the sum of the rest
 // at once; the number of any other is noted, some hundred of them in a row of any length.  These are looked at again with the last
 // bound: what reaches it is ranked by counting, and all but the first k join the sum.  Rows with more than these lists hold (plateaus
-// of equal values, rows that only ascend) take their bound by bisection instead, reading the row again and again.
+// of equal values, rows that only ascend, rows full of NaN) take their bound by bisection instead, reading the row again and again.
+// Masked rows: what is -inf or the type's lowest number is below every bound.  While fewer than k threads have met more than that,
+// the bound is looked for at every tile; where the row's other numbers do not fill the list, its first k classes have as many of the
+// masked ones as it needs (in rows that hold both kinds of them perhaps not: bisection).  2 047 x 50 001 bf16, k = 64, all but 40 or
+// 1 000 of the classes masked, or half: 46 to 56 us (57 of evenly spread ones; by bisection 2 000).
 //   2 047 x 50 001 bf16, k = 64: reading the row a second time for the sum, from whatever cache has it, took 101 us, keeping it in
 //   registers (which leaves room for few workgroups) 222, collecting elements instead of units' numbers 88.
 template <int G> struct alignas(16) TopShared {
-    static constexpr int parts = G < 256 ? G : 256, notes = G == 64 ? 256 : 2048;       // G = 64: up to 256 units
+    static constexpr int parts = G < 256 ? G : 256, notes = G == 64 ? 256 : 2048;       // more than evenly spread rows need
     static constexpr int room = G == 64 ? 256 : 1024;
     unsigned long long cand[room];              // (order, ~class): no two are equal
-    uint32_t most[parts];
+    uint32_t most[G];
     double redd[G / 64];
     long long redi[G / 64];
     float redf[G / 64];
@@ -211,7 +215,27 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
     const Scale scale = scale_of<T>(temperature);
     if (t == 0) s.count = s.noted = 0;
 
+    constexpr float LOWEST = sizeof(T) == 4 ? -3.402823466e38f : std::is_same<T, pxg_f16>::value ? -65504.f : -3.3895313892515355e38f;
+    const uint32_t MASKED = order_of(LOWEST);
     float largest = -INFINITY, bound = 0.f;
+    const auto search = [&](auto parts) {       // the k-th largest of `most`: one wave, bit by bit; one that is a little low will do
+        constexpr int P = decltype(parts)::value;
+        if (t < 64) {
+            uint32_t o[P / 64];
+#pragma unroll
+            for (int j = 0; j < P / 64; j++) o[j] = s.most[t + 64 * j];
+            uint32_t key = 0;
+            for (int bit = 31; bit >= 14; bit--) {
+                const uint32_t more = key | 1u << bit;
+                int c = 0;
+#pragma unroll
+                for (int j = 0; j < P / 64; j++) c += __popcll(__ballot(o[j] >= more));
+                if (c >= k) key = more;
+            }
+            if (t == 0) s.bound = key;
+        }
+        group_sync<G>();
+    };
     const auto raise_bound = [&] {              // the k-th largest of the threads' maxima
         float m = largest;
 #pragma unroll
@@ -219,22 +243,16 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
         group_sync<G>();
         if (t % EACH == 0) s.most[t / EACH] = order_of(m);
         group_sync<G>();
-        if (t < 64) {                           // one wave, bit by bit; a bound that is a little low will do
-            uint32_t o[PARTS / 64];
-#pragma unroll
-            for (int j = 0; j < PARTS / 64; j++) o[j] = s.most[t + 64 * j];
-            uint32_t key = 0;
-            for (int bit = 31; bit >= 14; bit--) {
-                const uint32_t more = key | 1u << bit;
-                int c = 0;
-#pragma unroll
-                for (int j = 0; j < PARTS / 64; j++) c += __popcll(__ballot(o[j] >= more));
-                if (c >= k) key = more;
-            }
-            if (t == 0) s.bound = key;
+        search(std::integral_constant<int, PARTS>());
+        uint32_t key = s.bound;
+        if (EACH > 1 && key <= MASKED) {         // a few hundred numbers in a row lie with a few threads: each for itself
+            group_sync<G>();
+            s.most[t] = order_of(largest);
+            group_sync<G>();
+            search(std::integral_constant<int, G>());
+            key = s.bound;
         }
-        group_sync<G>();
-        bound = value_of(s.bound);
+        bound = value_of(key > MASKED ? key : MASKED + 1);
     };
     RunningSum<T> sum;
     const auto take = [&](const float (&v)[n], int64_t unit) {
@@ -277,10 +295,11 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
 #pragma unroll
                 for (int e = 0; e < n; e++) largest = larger(largest, v[e]);
             }
-            if (tile++ == next) {               // tiles 0, 1, 2, 3, 4, 6, 9, 13, ...
-                next += next / 2 + (next < 2 ? 1 : 0);
+            if (tile == next || s.bound <= MASKED) {          // tiles 0, 1, 2, 3, 4, 6, 9, 13, ...
+                if (tile == next) next += next / 2 + (next < 2 ? 1 : 0);
                 raise_bound();
             }
+            tile++;
 #pragma unroll
             for (int a = 0; a < AHEAD; a++) {
                 float v[n];
@@ -311,6 +330,22 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
         }
     group_sync<G>();
     int found = listed ? s.count : CAND + 1;
+    double listed_lowest = 0.0;                 // of the sum so far
+    if (found < k) {                            // all that was summed is masked: the first ones fill the list
+        const bool lowest = group_reduce<G>((int)(sum.sum > 0.f || most > -INFINITY), s.red, MaxOf());
+        const float fill = lowest ? LOWEST : -INFINITY;
+        const int need = k - found;
+        group_sync<G>();
+        for (int i = t; i < k; i += G) {
+            if (pxg_to_f32(x[i]) != fill) continue;
+            int before = 0;
+            for (int j = 0; j < i; j++) before += pxg_to_f32(x[j]) == fill;
+            if (before < need) s.cand[atomicAdd(&s.count, 1)] = (unsigned long long)order_of(fill) << 32 | (uint32_t)~(uint32_t)i;
+        }
+        group_sync<G>();
+        found = s.count == k ? k : CAND + 1;
+        listed_lowest = lowest ? need : 0;
+    }
     bool no_number = false;                     // among the rest (bisection only: otherwise it is a candidate)
     if (found > CAND) {
         // the largest key that k elements reach, bit by bit; then the smallest class below which enough of the ties lie
@@ -335,7 +370,7 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
             if (count([&](uint32_t o, uint32_t c) { return o == key && c < mid; }) >= need) high = mid;
             else low = mid;
         }
-        found = k, listed = false, most = -INFINITY;
+        found = k, listed = false, most = -INFINITY, listed_lowest = 0.0;
         if (t == 0) s.count = 0;
         group_sync<G>();
         sum = RunningSum<T>();
@@ -372,6 +407,7 @@ void k_top(int64_t rows, int64_t classes, const T* logits, int64_t row_stride, i
         }
         below += (double)group_reduce<G>(parts, s.redi, SumOf()) * 0x1p-44;
     }
+    below -= listed_lowest;                     // (each counts 1: nothing larger is in the sum)
     // rank the candidates; the first k are the answer, the rest join the sum against the largest of them
     long long extra = 0;
     const bool left = found > k;

@@ -718,6 +718,73 @@ def test_top_logits_of_many_rows(rows, classes, k, dtype):
     check_top(x.to(TYPES[dtype]), k, 1.0)
 
 
+def masked_rows(rows, classes, k, dtype, seed=46):
+    """rows of numbers where a mask leaves none to all of them, in one piece, scattered, or at the places of one thread"""
+    g = torch.Generator().manual_seed(seed + classes)
+    low = torch.finfo(TYPES[dtype]).min
+    x, r = torch.full((rows, classes), -math.inf), 0
+    for count in sorted({min(c, classes) for c in (0, 1, 2, k - 1, k, k + 1, 130, 500, 2000, 5000)}):
+        places = [torch.arange(count), classes - count + torch.arange(count), (classes - count) // 2 + torch.arange(count),
+                  torch.randperm(classes, generator=g)[:count], (torch.arange(count) * 4096) % classes + torch.arange(count) * 4096 // classes]
+        for at in places:
+            at = at.unique().clamp(max=classes - 1)
+            x[r, :] = -math.inf if r % 2 else low                   # the type's lowest number masks as well, and is a number
+            x[r, at] = torch.randn(len(at), generator=g) * 3
+            r += 1
+    x[r] = low
+    x[r + 1, classes // 2:] = low                                   # both kinds
+    x[r + 2, :classes // 2] = low
+    x[r + 3, 1::2], x[r + 3, 4] = low, 1.0
+    x[r + 4, classes // 3], x[r + 4, classes - 1] = math.inf, math.nan
+    x[r + 5, -3:] = low
+    x[r + 6:] = torch.randn(rows - r - 6, classes, generator=g)
+    x[r + 6:, :classes // 2] = -math.inf
+    return x.to(TYPES[dtype])
+
+
+@gpu
+@pytest.mark.parametrize('rows,classes,k,dtype', [(60, 700, 9, 'f32'), (60, 5003, 128, 'bf16'), (70, 30001, 100, 'bf16'), (80, 40000, 128, 'f32'),
+                                                  (1100, 3001, 64, 'f32'), (1100, 9001, 50, 'f16'), (2050, 5003, 31, 'f32'),
+                                                  (2050, 3001, 1, 'f16')])
+def test_top_logits_of_masked_rows(rows, classes, k, dtype):
+    x = masked_rows(rows, classes, k, dtype)
+    check_top(x, k, 1.0)
+    # the rest of each row by what its own numbers allow (check_top goes by the largest of all): masked places add nothing beside
+    # others, and count one each where they are all that is left
+    got, rest = ops.top_logits(x.cuda(), k, 1.0).rest.double().cpu().numpy(), top_statement(x.double().numpy(), k, 1.0)[2]
+    for r in range(rows):
+        if np.isfinite(rest[r]):
+            own = x[r][torch.isfinite(x[r]) & (x[r] > torch.finfo(x.dtype).min)].double().abs()
+            most = float(own.max()) if len(own) else 0.0
+            assert abs(got[r] - rest[r]) <= 2.0 ** -24 * (abs(rest[r]) + 64 + 2 * most), r
+
+
+@gpu
+@pytest.mark.parametrize('rows,classes,k,dtype', [(2047, 50001, 64, 'bf16'), (500, 131071, 100, 'f32'), (4096, 8000, 8, 'f16'), (100, 60001, 128, 'bf16')])
+def test_masked_rows_take_one_pass(rows, classes, k, dtype):
+    """masks that leave a few, a thousand or half of the classes: not ten times the work (bisection takes thirty)"""
+    x = torch.randn(rows, classes, device='cuda', generator=torch.Generator('cuda').manual_seed(47)).to(TYPES[dtype])
+
+    def time_of(x):
+        ops.top_logits(x, k)
+        times = []
+        for _ in range(5):
+            begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            begin.record()
+            for _ in range(5):
+                ops.top_logits(x, k)
+            end.record()
+            torch.cuda.synchronize()
+            times.append(begin.elapsed_time(end) / 5)
+        return min(times)
+    free = time_of(x)
+    for mask in (-math.inf, torch.finfo(x.dtype).min):
+        for keep in (slice(0, 40), slice(classes // 3, classes // 3 + 1000), slice(classes // 2, classes)):
+            masked = torch.full_like(x, mask)
+            masked[:, keep] = x[:, keep]
+            assert time_of(masked) < 8 * free, (mask, keep)
+
+
 @gpu
 @pytest.mark.parametrize('rows,classes,k,dtype', [(4096, 2047, 5, 'f32'), (4099, 1500, 100, 'bf16')])
 def test_distillation_loss_of_many_rows(rows, classes, k, dtype):
