@@ -174,16 +174,23 @@ def weighted_accuracy(logp, labels, cost):
 
 def distillation_targets(teacher, x, k=3, temperature=2.0, device='cuda', batch_size=4096):
     """The teacher's `k` largest answers to every sample of x (torch_ops.TopLogits on the CPU): the targets of
-    ``Trainer(model, torch_ops.distillation_loss).fit(x, targets)``."""
+    ``Trainer(model, torch_ops.distillation_loss).fit(x, targets)``.  The teacher is moved to `device`, as ``Trainer`` moves its
+    model, and answers in evaluation mode; its modules' modes come back."""
     from . import torch_ops
     if len(x) == 0:
         raise ValueError('no samples to ask the teacher about')
     device, parts = torch.device(device), []
-    teacher = teacher.to(device).eval()
-    with torch.no_grad():
-        for a in range(0, len(x), batch_size):
-            logits = teacher(x[a:a + batch_size].to(device))
-            parts.append(torch_ops.top_logits(logits, min(k, logits.shape[1]), temperature).to('cpu'))
+    teacher = teacher.to(device)
+    modes = [(m, m.training) for m in teacher.modules()]
+    try:
+        teacher.eval()
+        with torch.no_grad():
+            for a in range(0, len(x), batch_size):
+                logits = teacher(x[a:a + batch_size].to(device))
+                parts.append(torch_ops.top_logits(logits, min(k, logits.shape[1]), temperature).to('cpu'))
+    finally:
+        for m, training in modes:
+            m.training = training
     return torch_ops.TopLogits.cat(parts)
 
 

@@ -43,6 +43,19 @@ def test_no_samples_and_no_answers_are_refused():
         ops.TopLogits.cat([])
 
 
+def test_the_teachers_modes_come_back(monkeypatch):
+    monkeypatch.setattr(ops, 'top_logits', lambda x, k, tau: ops.TopLogits(x[:, :k], torch.arange(k).repeat(len(x), 1), x[:, -1], tau))
+    teacher = TR.DemuxClassifier().train()
+    teacher.drop1.eval()
+    modes, x = [m.training for m in teacher.modules()], torch.randn(7, 300)
+    first = TR.distillation_targets(teacher, x, device='cpu', batch_size=4)
+    assert [m.training for m in teacher.modules()] == modes and len(first) == 7
+    assert first.values.equal(TR.distillation_targets(teacher, x, device='cpu').values)          # in evaluation mode: no dropout
+    with pytest.raises(ValueError, match='LSTM'):
+        TR.distillation_targets(teacher, x[:, :, None, None], device='cpu')
+    assert [m.training for m in teacher.modules()] == modes
+
+
 def test_trainer_takes_top_logits(tmp_path):
     """Targets that are TopLogits go through the trainer's split, shuffling and batches like labels: every sample meets its own."""
     n = 70
