@@ -18,6 +18,7 @@ Arguments are checked here; csrc/pxg_torch.cpp makes the calls and is the autogr
 import ctypes as C
 import importlib.machinery
 import importlib.util
+import numbers
 import operator
 import os
 
@@ -173,8 +174,10 @@ class TopLogits:
         return len(self.values)
 
     def __getitem__(self, rows):
-        if isinstance(rows, int):
-            rows = slice(rows, rows + 1 or None)
+        if isinstance(rows, numbers.Integral):
+            if not -len(self) <= rows < len(self):
+                raise IndexError('row {} of {}'.format(rows, len(self)))             # what ends a loop over the rows
+            rows = slice(int(rows), int(rows) + 1 or None)
         return TopLogits(self.values[rows], self.indices[rows], None if self.rest is None else self.rest[rows], self.temperature)
 
     def to(self, *args, **kwargs):

@@ -1213,6 +1213,19 @@ def test_recordings_are_refused_on_the_gpu():
     assert torch.equal(got, want)
 
 
+def test_answers_one_row_after_the_other():
+    t = ops.TopLogits(torch.arange(8.0).view(4, 2), torch.arange(8).view(4, 2), torch.arange(4.0), 2.0)
+    rows = []
+    for row in t:
+        rows.append(row)
+        assert len(rows) <= 4
+    assert ops.TopLogits.cat(rows).values.equal(t.values) and ops.TopLogits.cat(rows).rest.equal(t.rest)
+    assert t[np.int64(2)].values.equal(t.values[2:3]) and t[np.int64(-1)].rest.equal(t.rest[3:])
+    for at in (4, -5, np.int64(4)):
+        with pytest.raises(IndexError, match='of 4'):
+            t[at]
+
+
 def mixed_parts():
     x, t, weight = distill_problem(6, 40, 3, 'f32', 2.0, seed=41)
     return x, weight, [t[:2], ops.TopLogits(t.values[2:5], t.indices[2:5], None, 2.0), t[5:]], t
