@@ -964,6 +964,7 @@ class NativeContext:
             self._unlocked.add(_ptr(array).value)
             return array
         self._check(rc, 'pxg_host_register')
+        getattr(self, '_unlocked', set()).discard(_ptr(array).value)       # (of an array that was here before and never unpinned)
         self._pinned = getattr(self, '_pinned', {})
         self._pinned[_ptr(array).value] = array       # (kept alive until it is released)
         return array

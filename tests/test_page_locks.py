@@ -48,6 +48,15 @@ def test_an_array_that_is_not_locked_stays_usable():
     assert ctx.lib.released == [array.ctypes.data]
 
 
+def test_a_lock_is_released_whatever_was_refused_at_its_address():
+    ctx, array = context(native.PXG_E_UNSUPPORTED), pages()
+    ctx.pin(array)                                     # refused, and gone without unpin()
+    ctx.lib.code = 0
+    ctx.pin(array)                                     # what is mapped there now is locked
+    ctx.unpin(array)
+    assert ctx.lib.released == [array.ctypes.data] and not ctx._pinned and not ctx._unlocked
+
+
 def test_other_errors_are_raised():
     with pytest.raises(native.PxgError, match='the reason'):
         context(-3).pin(pages())
