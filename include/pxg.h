@@ -363,7 +363,8 @@ int pxg_batch_swap(pxg_ctx* ctx);
  * memory of the caller; the runtime's own in-place lock of such a source is what took the process down in round 4:
  * INTEGRATION.md section 2).  Register MAPPED pages of their own (mmap), never a slice of a malloc'ed block: a
  * brk-heap range that was page-locked once must not be page-locked again later in the process.
- * PXG_E_UNSUPPORTED: this machine locks no memory that already exists; the range stays pageable and usable.
+ * PXG_E_INVALID: part of the range is not mapped.  PXG_E_UNSUPPORTED: this machine locks no memory that already exists (it refuses
+ * a page of the library's own as well); the range stays pageable and usable.  PXG_E_HIP: any other refusal.
  * pxg_host_unregister accepts ctx == NULL: page locks are process-wide, and a range may have to be released after the
  * context that registered it is gone (a staging arena must not be unmapped while it is still registered). */
 int pxg_host_register(pxg_ctx* ctx, void* ptr, size_t bytes);

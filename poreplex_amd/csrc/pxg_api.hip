@@ -8,6 +8,8 @@
 #include <chrono>
 #include <stdio.h>
 #include <stdlib.h>
+#include <sys/mman.h>
+#include <unistd.h>
 #include "pxg_common.h"
 #include <cctype>
 #include "pxg_zcheck.h"
@@ -763,16 +765,43 @@ extern "C" int pxg_batch_swap(pxg_ctx* ctx)
     return PXG_OK;
 }
 
+// whether this process has something mapped at every page of the range (MS_ASYNC writes nothing: it walks the mappings)
+static bool range_is_mapped(const void* ptr, size_t bytes)
+{
+    const uintptr_t page = (uintptr_t)sysconf(_SC_PAGESIZE), first = (uintptr_t)ptr / page * page;
+    if ((uintptr_t)ptr + bytes < (uintptr_t)ptr) return false;
+    return msync((void*)first, (uintptr_t)ptr + bytes - first, MS_ASYNC) == 0;
+}
+
+// Whether this machine page-locks memory that already exists, found out on a page of our own: some refuse any with the error that
+// also stands for a wrong address or size.
+static bool machine_locks_memory()
+{
+    static const bool locks = [] {
+        const size_t page = (size_t)sysconf(_SC_PAGESIZE);
+        void* own = mmap(nullptr, page, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
+        if (own == MAP_FAILED) return true;              // not known: an error is then reported as one
+        memset(own, 0, page);
+        const bool got = hipHostRegister(own, page, hipHostRegisterDefault) == hipSuccess;
+        // (a page that cannot be released stays mapped: a registration of memory that is gone is worse than a lost page)
+        if (got && hipHostUnregister(own) != hipSuccess) { (void)hipGetLastError(); return true; }
+        if (!got) (void)hipGetLastError();
+        munmap(own, page);
+        return got;
+    }();
+    return locks;
+}
+
 extern "C" int pxg_host_register(pxg_ctx* ctx, void* ptr, size_t bytes)
 {
-    if (!ctx || !ptr || !bytes) return PXG_E_INVALID;
+    if (!ctx || !ptr || !bytes || !range_is_mapped(ptr, bytes)) return PXG_E_INVALID;
     PXG_HIP(ctx, hipSetDevice(ctx->device));
     const hipError_t e = hipHostRegister(ptr, bytes, hipHostRegisterDefault);
     if (e == hipSuccess) return PXG_OK;
     (void)hipGetLastError();                     // or the next call on any stream would report it as its own
     pxg_set_err(ctx, std::string("hipHostRegister: ") + hipGetErrorString(e));
-    // some machines lock no memory that already exists: the copies then go through the context's own page-locked chunks
-    return e == hipErrorInvalidValue || e == hipErrorNotSupported ? PXG_E_UNSUPPORTED : PXG_E_HIP;
+    // a machine that locks none: the copies then go through the context's own page-locked chunks
+    return (e == hipErrorInvalidValue || e == hipErrorNotSupported) && !machine_locks_memory() ? PXG_E_UNSUPPORTED : PXG_E_HIP;
 }
 
 extern "C" int pxg_host_unregister(pxg_ctx* ctx, void* ptr)

@@ -7,6 +7,7 @@ no GPU is usable this module fails LOUDLY -- there is no CPU fallback.
 """
 import ctypes as C
 import os
+import warnings
 
 import numpy as np
 
@@ -382,6 +383,7 @@ class NativeConfig:
 # library loading
 # --------------------------------------------------------------------------
 _lib = None
+_warned_of_pageable = False
 
 TEXT_LIB_PATH = os.path.join(HERE, 'csrc', 'libpxghost.so')
 _TEXT_SIGNATURES = {      # libpxghost.so: host-only helpers (sink text, sample codec)
@@ -957,11 +959,17 @@ class NativeContext:
 
     def pin(self, array):
         """Page-lock a NumPy array so stage() copies are DMA transfers; returns it.  Where the machine locks no
-        memory that already exists the array stays pageable: slower copies, the same results."""
+        memory that already exists the array stays pageable: slower copies, the same results, and a RuntimeWarning
+        (the first time in a process)."""
+        global _warned_of_pageable
         rc = self.lib.pxg_host_register(self.handle, _ptr(array), array.nbytes)
         if rc == PXG_E_UNSUPPORTED:
             self._unlocked = getattr(self, '_unlocked', set())
             self._unlocked.add(_ptr(array).value)
+            if not _warned_of_pageable:
+                _warned_of_pageable = True
+                warnings.warn('this machine page-locks no memory that already exists: arrays stay pageable, and their copies to '
+                              'and from the GPU are slower', RuntimeWarning, stacklevel=2)
             return array
         self._check(rc, 'pxg_host_register')
         getattr(self, '_unlocked', set()).discard(_ptr(array).value)       # (of an array that was here before and never unpinned)

@@ -57,6 +57,16 @@ def test_a_lock_is_released_whatever_was_refused_at_its_address():
     assert ctx.lib.released == [array.ctypes.data] and not ctx._pinned and not ctx._unlocked
 
 
+def test_arrays_that_stay_pageable_are_said_to(monkeypatch):
+    monkeypatch.setattr(native, '_warned_of_pageable', False, raising=False)
+    with pytest.warns(RuntimeWarning, match='pageable') as seen:
+        for _ in range(3):
+            ctx, array = context(native.PXG_E_UNSUPPORTED), pages()
+            ctx.pin(array)
+            ctx.unpin(array)
+    assert len(seen) == 1                              # once in a process
+
+
 def test_other_errors_are_raised():
     with pytest.raises(native.PxgError, match='the reason'):
         context(-3).pin(pages())
@@ -71,4 +81,19 @@ def test_a_refused_lock_leaves_no_error_behind():
     ctx.unpin(array)
     other = native.NativeContext(default_config())     # a stale error would end this call
     other.close()
+    ctx.close()
+
+
+@pytest.mark.gpu
+def test_a_wrong_range_is_an_error_of_its_own():
+    from poreplex_amd.config import default_config
+    ctx = native.NativeContext(default_config())
+    array = pages()
+    register = ctx.lib.pxg_host_register
+    for at, size in ((array.ctypes.data, 1 << 40), (4096, 4096), (array.ctypes.data, (1 << 64) - 1)):    # not mapped (all of it)
+        assert register(ctx.handle, at, size) == -1
+    rc = register(ctx.handle, array.ctypes.data, array.nbytes)
+    assert rc in (0, native.PXG_E_UNSUPPORTED)
+    if rc == 0:
+        assert ctx.lib.pxg_host_unregister(ctx.handle, array.ctypes.data) == 0
     ctx.close()
