@@ -1037,8 +1037,7 @@ int pxg_d2h_sync(pxg_ctx* ctx, void* dst, const void* src, size_t bytes)
 int pxg_h2d_big(pxg_ctx* ctx, void* dst, const void* src, size_t bytes, hipStream_t st)
 {
     if (!bytes) return PXG_OK;
-    // (PXG_H2D_RUNTIME_LOCKS=1: the round-4 behaviour, for tools/heap_pin_fault.py to show what it leads to)
-    if (bytes < (512u << 10) || getenv("PXG_H2D_RUNTIME_LOCKS")) {       // staged by the runtime through ITS page-locked buffer
+    if (bytes < (512u << 10)) {       // staged by the runtime through ITS page-locked buffer
         PXG_HIP(ctx, hipMemcpyAsync(dst, src, bytes, hipMemcpyHostToDevice, st));
         return PXG_OK;
     }

@@ -1,5 +1,6 @@
 """Host arrays on machines that lock no memory that already exists: pin() leaves them pageable, unpin() takes them back."""
 import mmap
+import os
 
 import numpy as np
 import pytest
@@ -65,6 +66,25 @@ def test_arrays_that_stay_pageable_are_said_to(monkeypatch):
             ctx.pin(array)
             ctx.unpin(array)
     assert len(seen) == 1                              # once in a process
+
+
+def test_pageable_memory_has_no_way_to_the_runtime():
+    """The runtime's own lock of a pageable range can end the process in a GPU memory fault: no switch leads there, and nothing in the
+    tree builds device code for, or repeats runs until, such a fault."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    csrc = os.path.join(root, 'poreplex_amd', 'csrc')
+    with open(os.path.join(csrc, 'pxg_api.hip')) as f:
+        source = f.read()
+    begin = source.index('int pxg_h2d_big(')
+    assert 'getenv("PXG_H2D' not in source and 'LOCKS")' not in source[begin:source.index('\n}\n', begin)]
+    with open(os.path.join(csrc, 'Makefile')) as f:
+        assert 'xnack' not in f.read()
+    for folder, _, names in os.walk(os.path.join(root, 'tools')):
+        for name in names:
+            assert not name.endswith('hunt.sh')
+            if name.endswith(('.sh', '.py')):
+                with open(os.path.join(folder, name)) as f:
+                    assert 'HSA_XNACK' not in f.read(), name
 
 
 def test_other_errors_are_raised():
