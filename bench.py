@@ -77,6 +77,45 @@ STAGES = {
 }
 
 
+MOST_BYTES = 16000           # of the line: what collects it may keep the end of a longer one only (25 KB came through cut)
+
+
+def short(x):
+    """Floats below the top level to six digits."""
+    if isinstance(x, float):
+        return float('{:.6g}'.format(x))
+    if isinstance(x, dict):
+        return {k: short(v) for k, v in x.items()}
+    return [short(v) for v in x] if isinstance(x, list) else x
+
+
+def emit(json_fd, line, record=None):
+    """The one JSON line.  Where it would be too long, copies of committed files go first, then the largest entries of `extra`;
+    `extra.left_out` names them.  `record`: a file that gets all of it (--record)."""
+    out, left = {k: short(v) if isinstance(v, (dict, list)) else v for k, v in line.items()}, []
+
+    def text():
+        return (json.dumps(out) + '\n').encode()
+    flips = (out.get('concordance') or {}).get('unpinned_decision_flips')
+    if len(text()) > MOST_BYTES and flips:
+        out['concordance']['unpinned_decision_flips'] = {k: v.get('source') for k, v in flips.items()}
+        left.append('concordance.unpinned_decision_flips')
+    extra = out.get('extra') or {}
+    for key in sorted(extra, key=lambda k: -len(json.dumps(extra[k]))):
+        if len(text()) <= MOST_BYTES - 400:
+            break
+        left.append(key)
+        del extra[key]
+    if left:
+        out['extra'] = dict(extra, left_out=left)
+    if record:
+        with open(record, 'w') as fh:
+            json.dump(line, fh)
+    data = text()
+    while data:                                        # (a pipe may take less at once)
+        data = data[os.write(json_fd, data):]
+
+
 def parse(argv=None):
     ap = argparse.ArgumentParser()
     ap.add_argument('--gpus', type=int, default=1)
@@ -141,6 +180,8 @@ def parse(argv=None):
                     help='API leg: skip the 128-read calls from 8 / 14 worker PROCESSES (the reference\'s ProcessPoolExecutor pattern)')
     ap.add_argument('--no-latency-leg', action='store_true',
                     help='skip the small-batch leg (roofline.latency_form: a 1 024-read batch with and without the latency forms of K2 / K5)')
+    ap.add_argument('--record', metavar='FILE', help='write the whole record there: the line leaves out what would make it longer than '
+                                                     '{} bytes'.format(MOST_BYTES))
     return ap.parse_args(argv)
 
 
@@ -348,7 +389,7 @@ def end_to_end(args, config, rank, local_rank, world, dist, standin, base, which
                           'host_us_per_read_rank0': round((out['timing']['facade_s'] + out['timing']['sink_s'])
                                                           / max(out['reads_this_rank'], 1) * 1e6, 2)},
             }
-            os.write(json_fd, (json.dumps(line) + '\n').encode())
+            emit(json_fd, line, args.record)
         WorkerPersistenceStorage.reset()
     finally:
         shutil.rmtree(work, ignore_errors=True)
@@ -1776,7 +1817,7 @@ def main():
                                        '(best of raw / encoded bundle: {:.0f} reads/s)'.format(
                                            api['raw']['calls'], api['raw']['reads_per_call'],
                                            api['raw']['in_flight'], best['reads_per_s']))
-    os.write(json_fd, (json.dumps(line) + '\n').encode())
+    emit(json_fd, line, args.record)
     if dist is not None:
         dist.destroy_process_group()
 
