@@ -237,6 +237,7 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
     constexpr bool APART = SLOPE && NP == 3;
     constexpr int KEEP_S = DOT ? 2 : KEEP;                    // of the state against x: the gradient of log_decay is made of them, too
     static_assert(PIECES * N == C * (D / 8), "whole pieces");
+    static_assert(C == 32, "a chunk is one operand of a matrix instruction: two tiles of 16 steps");
     const int bh = xcd_order(blockIdx.x, gridDim.x), b = bh / a.heads, h = bh % a.heads, seg = blockIdx.y;
     const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, g = lane / 16, li = lane % 16, f0 = wave * 16;
     const int E = r.E, F = r.F;
@@ -518,80 +519,75 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
                     S[t] *= decay;
                 }
             }
+            bf16x8 zw[3], zs[SLOPE ? SLOPE_PLANES : 1];
+            bf16x4 u[CT][3], v[CT][SLOPE ? SLOPE_PLANES : 1];
 #pragma unroll
-            for (int k = 0; k < C / 32; k++) {
-                static_assert(C == 32 || !APART, "the state decays once a chunk");
-                bf16x8 zw[3], zs[SLOPE ? SLOPE_PLANES : 1];
-                bf16x4 u[2][3], v[2][SLOPE ? SLOPE_PLANES : 1];
+            for (int jt = 0; jt < CT; jt++) {
+                const __bf16* at = tz + jt * 16 * ROW + f0 + at_tr;
+                f32x4 value = widen(read_transposed(at + (NP - 1) * PLANE));
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    const int jt = 2 * k + half;
-                    const __bf16* at = tz + jt * 16 * ROW + f0 + at_tr;
-                    f32x4 value = widen(read_transposed(at + (NP - 1) * PLANE));
+                for (int n = NP - 2; n >= 0; n--) value += widen(read_transposed(at + n * PLANE));
+                value *= w_state;
+                if (jt < CT - 1) value *= tiles[CT - 1 - jt];
+                split<3>(value, u[jt]);
+                if constexpr (SLOPE) {
 #pragma unroll
-                    for (int n = NP - 2; n >= 0; n--) value += widen(read_transposed(at + n * PLANE));
-                    value *= w_state;
-                    if (jt < CT - 1) value *= tiles[CT - 1 - jt];
-                    split<3>(value, u[half]);
-                    if constexpr (SLOPE) {
+                    for (int n = 0; n < 4; n++) value[n] *= (float)(C - 1 - jt * 16 - 4 * g - n);
+                    split<SLOPE_PLANES>(value, v[jt]);
+                }
+            }
 #pragma unroll
-                        for (int n = 0; n < 4; n++) value[n] *= (float)(C - 1 - jt * 16 - 4 * g - n);
-                        split<SLOPE_PLANES>(value, v[half]);
-                    }
+            for (int p = 0; p < 3; p++) zw[p] = join(u[0][p], u[1][p]);
+            if constexpr (SLOPE)
+#pragma unroll
+                for (int p = 0; p < SLOPE_PLANES; p++) zs[p] = join(v[0][p], v[1][p]);
+#pragma unroll
+            for (int t = 0; t < ET; t++) {
+                bf16x8 yt[NP];
+#pragma unroll
+                for (int n = 0; n < NP; n++) {
+                    const __bf16* at = ty + n * PLANE + t * 16 + at_tr;
+                    yt[n] = join(read_transposed(at), read_transposed(at + 16 * ROW));
+                }
+                f32x4 sum = {}, slope = {};
+                if constexpr (!APART) {
+                    sum = S[t];
+                    if constexpr (SLOPE) slope = G[t];
                 }
 #pragma unroll
-                for (int p = 0; p < 3; p++) zw[p] = join(u[0][p], u[1][p]);
-                if constexpr (SLOPE)
+                for (int p = 2; p >= 0; p--)
 #pragma unroll
-                    for (int p = 0; p < SLOPE_PLANES; p++) zs[p] = join(v[0][p], v[1][p]);
+                    for (int n = 0; n < NP; n++)
+                        if (p + n <= 2) sum = mfma(yt[n], zw[p], sum);
+                if constexpr (SLOPE) {
 #pragma unroll
-                for (int t = 0; t < ET; t++) {
-                    bf16x8 yt[NP];
-#pragma unroll
-                    for (int n = 0; n < NP; n++) {
-                        const __bf16* at = ty + n * PLANE + k * 32 * ROW + t * 16 + at_tr;
-                        yt[n] = join(read_transposed(at), read_transposed(at + 16 * ROW));
-                    }
-f32x4 sum = {}, slope = {};
-                    if constexpr (!APART) {
-                        sum = S[t];
-                        if constexpr (SLOPE) slope = G[t];
-                    }
-#pragma unroll
-                    for (int p = 2; p >= 0; p--)
+                    for (int p = SLOPE_PLANES - 1; p >= 0; p--)
 #pragma unroll
                         for (int n = 0; n < NP; n++)
-                            if (p + n <= 2) sum = mfma(yt[n], zw[p], sum);
-                    if constexpr (SLOPE) {
-#pragma unroll
-                        for (int p = SLOPE_PLANES - 1; p >= 0; p--)
-#pragma unroll
-                            for (int n = 0; n < NP; n++)
-                                if (p + n < SLOPE_PLANES) slope = mfma(yt[n], zs[p], slope);
-                        G[t] = APART ? (G[t] + S[t] * (float)(C - skip)) * decay + slope : slope;
-                    }
-                    S[t] = APART ? S[t] * decay + sum : sum;
+                            if (p + n < SLOPE_PLANES) slope = mfma(yt[n], zs[p], slope);
+                    G[t] = APART ? (G[t] + S[t] * (float)(C - skip)) * decay + slope : slope;
                 }
+                S[t] = APART ? S[t] * decay + sum : sum;
             }
         }
         if constexpr (OUT && W > 1) __syncthreads();          // the weights are there
         if (OUT && works) {
-            // P z, 32 earlier steps at a time
-            const auto add_block = [&](int it, int k, auto careful) {
+            // P z
+            const auto add_rows = [&](int it, auto careful) {
                 bf16x8 wp[KEEP + 1], zb[NP];
 #pragma unroll
                 for (int p = 0; p <= KEEP; p++) {
                     if constexpr (W == 1) {
-                        const int n = it * (it + 1) / 2 + 2 * k;
-                        wp[p] = join(own[n][p], 2 * k + 1 <= it ? own[n + 1][p] : bf16x4{});
+                        const int n = it * (it + 1) / 2;
+                        wp[p] = join(own[n][p], it > 0 ? own[n + 1][p] : bf16x4{});
                     } else {
-                        const __bf16* at = weights + p * PPLANE + (it * 16 + li) * PROW + k * 32 + 4 * g;
-                        wp[p] = join(*(const bf16x4*)at, 2 * k + 1 <= it ? *(const bf16x4*)(at + 16) : bf16x4{});
+                        const __bf16* at = weights + p * PPLANE + (it * 16 + li) * PROW + 4 * g;
+                        wp[p] = join(*(const bf16x4*)at, it > 0 ? *(const bf16x4*)(at + 16) : bf16x4{});
                     }
                 }
 #pragma unroll
                 for (int n = 0; n < NP; n++) {
-                    const __bf16* at = tz + n * PLANE + k * 32 * ROW + f0 + at_tr;
+                    const __bf16* at = tz + n * PLANE + f0 + at_tr;
                     zb[n] = join(read_transposed(at), read_transposed(at + 16 * ROW));
                 }
                 const auto add = [&](const bf16x8* zz, f32x4 to) {
@@ -612,7 +608,7 @@ f32x4 sum = {}, slope = {};
                         for (int n = 0; n < NP; n++)
 #pragma unroll
                             for (int m = 0; m < 8; m++) {
-                                const int j = (m / 4 - it % 2) * 16 + 4 * g + m % 4;             // from the tile's first row
+                                const int j = (m / 4 - it) * 16 + 4 * g + m % 4;             // from the tile's first row
                                 zz[n][m] = j <= i ? zb[n][m] : (__bf16)0.f;
                             }
                         const f32x4 one = add(zz, before);
@@ -624,16 +620,10 @@ f32x4 sum = {}, slope = {};
             };
             if (strange[c & 1]) {
 #pragma unroll
-                for (int it = 0; it < CT; it++) {
-#pragma unroll
-                    for (int k = 0; k < it / 2; k++) add_block(it, k, no);
-                    add_block(it, it / 2, yes);
-                }
+                for (int it = 0; it < CT; it++) add_rows(it, yes);
             } else {
 #pragma unroll
-                for (int it = 0; it < CT; it++)
-#pragma unroll
-                    for (int k = 0; k <= it / 2; k++) add_block(it, k, no);
+                for (int it = 0; it < CT; it++) add_rows(it, no);
             }
         }
         if constexpr (DOT) total += (double)part, part = 0.f;
