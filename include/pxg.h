@@ -720,7 +720,8 @@ int pxg_top_logits(int32_t dtype, int64_t rows, int64_t classes, const void* log
  * rest NULL: the listed ones are all there is), q = the student's softmax(logits / temperature) over the same k + 1 classes;
  *     row_loss[n] = weight[n] temperature^2 sum p (log p - log q),       loss = sum of row_loss / (mean ? rows : 1)
  * An index of -1 is an empty place; a class listed more than once gets the sum of its shares; an index outside the classes
- * makes its row's loss and gradient NaN.  Rows of weight 0 and rows with nothing listed and no rest give 0 whatever they hold. */
+ * makes its row's loss and gradient NaN.  The backward pass takes what the forward pass took; an index that has become no class since
+ * then is passed over.  Rows of weight 0 and rows with nothing listed and no rest give 0 whatever they hold. */
 typedef struct {
     uint32_t struct_bytes;            /* sizeof(pxg_distill) */
     int32_t dtype;                    /* pxg_dtype of logits and grad_logits */

@@ -746,6 +746,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_backward(const px
             const float d = stats[STATS + i];
             if (d == INFINITY) continue;
             const int64_t at = row * k + i, index = a.indices_are_64 ? ((const int64_t*)a.indices)[at] : ((const int32_t*)a.indices)[at];
+            if (index < 0 || index >= a.classes) continue;        // not what the forward pass saw: no place in this row
             marks.add(index, n);
             g[index] = pxg_from_f32<T>((float)(factor * (double)d));
         }

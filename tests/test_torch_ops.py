@@ -918,6 +918,40 @@ def test_top_logits_gives_the_same_bits_again(rows, classes, k):
 
 
 @gpu
+@pytest.mark.parametrize('classes', [40, 5003, 20001])
+@pytest.mark.parametrize('wide', [False, True])
+def test_indices_that_changed_behind_the_forward_pass_stay_in_their_rows(classes, wide):
+    """the C entries: the backward pass bounds the indices it is given itself; a place that is gone counts among the unlisted"""
+    x, teacher, weight = distill_problem(9, classes, 3, 'f32', 2.0, seed=50)
+    x, teacher = x.cuda(), teacher.to('cuda')
+    indices = teacher.indices.long() if wide else teacher.indices.clone()
+    guard, lib = classes * 4, N.load_library()
+    held = torch.full((2 * guard + 9 * classes,), 7.0, device='cuda')
+    stats, row_loss, one = torch.empty(9, 4 + 3, device='cuda'), torch.empty(9, device='cuda'), torch.ones(9, device='cuda')
+    d = N.PxgDistill()
+    d.struct_bytes, d.rows, d.classes, d.row_stride, d.k, d.temperature = C.sizeof(d), 9, classes, classes, 3, 2.0
+    d.logits, d.values, d.indices, d.rest = (t.data_ptr() for t in (x, teacher.values, indices, teacher.rest))
+    d.indices_are_64, d.grad_per_row, d.row_loss, d.stats = int(wide), 1, row_loss.data_ptr(), stats.data_ptr()
+    d.grad_loss, d.grad_logits = one.data_ptr(), held.data_ptr() + 4 * guard
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.pxg_distill_forward(C.byref(d), stream) == 0 and lib.pxg_distill_backward(C.byref(d), stream) == 0
+    grad = held[guard:-guard].view(9, classes).clone()
+    want = ops.distillation_loss_and_gradient(x, teacher, None, 'none')
+    assert torch.equal(row_loss, want[0]) and torch.equal(grad, want[1])
+    gone = [(0, 0, classes), (3, 1, -1), (5, 2, -2), (8, 0, classes * 2), (8, 1, -classes)] + ([(6, 0, 1 << 40)] if wide else [])
+    for row, place, index in gone:
+        indices[row, place] = index
+    held.fill_(7.0)
+    assert lib.pxg_distill_backward(C.byref(d), stream) == 0
+    got = held[guard:-guard].view(9, classes)
+    assert (held[:guard] == 7.0).all() and (held[-guard:] == 7.0).all()
+    same = torch.ones_like(got, dtype=torch.bool)
+    for row, place, index in gone:
+        same[row, int(teacher.indices[row, place])] = False
+    assert torch.equal(got[same], grad[same]) and torch.isfinite(got).all()
+
+
+@gpu
 def test_more_rows_than_one_axis_of_a_grid_holds():
     rows = (1 << 26) + 5                                           # four to a workgroup of 256: 2^32 threads and more
     x = torch.randn(rows, 2, device='cuda', generator=torch.Generator('cuda').manual_seed(4))
