@@ -680,7 +680,8 @@ typedef struct {
  *     S_t = a_h S_(t-1) + k_t v_t^T        o_t = q_t S_t        S_(-1) = initial_state (0 where NULL)
  * Steps at or behind lengths[b] are neither read nor part of the state; their rows of `out` and of the gradients are 0.
  * A length below 0 counts as 0, one above `steps` as `steps`.  A log_decay above 0 grows; the results are numbers while
- * exp(log_decay * steps) is one. */
+ * exp(log_decay * steps) is one.  Sums and states are float32; products leave out what is below 2^-24 of a term, or 2^-17 where the
+ * result is rounded to bfloat16 or float16. */
 typedef struct {
     uint32_t struct_bytes;            /* sizeof(pxg_decay) */
     int32_t dtype;                    /* pxg_dtype of q, k, v, out, grad_out and the gradients of q, k, v */

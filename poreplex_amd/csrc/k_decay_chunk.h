@@ -16,8 +16,12 @@
 //
 // Precision.  A matrix instruction takes bfloat16 operands and adds in float32.  A float32 number is the sum of three bfloat16
 // ("planes"), a float16 number of two, both exactly: products of planes p, q are taken for p + q <= 2, which leaves 2^-24.
-// What is computed in float32 and goes into a product (P, S, the weighted z) is split in the same way: into three planes where the
-// result is float32, into two (2^-18 left) where it is rounded to half precision; the state itself always takes three.
+// What is computed in float32 and goes into a product is split in the same way.  The weighted z that the state is made of takes three
+// planes, and so do state and slope in the run that gives the gradient of log_decay.  The weights P, and the state as an operand
+// against x in all other runs, take three where the result is float32 and two (2^-18 left of each term) where it is rounded to half
+// precision: the errors against 64 bits are those of one rounding then as well (128 x 2 000 x 8 x 64: f16 2.074e-4, bf16 1.659e-3
+// either way), and three planes everywhere took 588 us instead of 537 (1 x 100 003 x 8 x 128 f16) and 221 instead of 210 (training
+// 16 x 2 000 x 8 x 64 bf16).  The state itself is float32 from the first chunk to the last.
 //
 // The gradient of log_decay: inside a chunk sum_{j < i} (i - j) P_ij (q_i . z_j), a second product of rows beside P; from earlier
 // chunks q_i . (x_i dS/dlog_decay), with the slope G = dS/dlog_decay carried like the state.
@@ -28,10 +32,11 @@
 // 0 * inf: a weight of 0 (j > i) does not keep a z that is no finite number out of a matrix product.  Staging looks for such z;
 // a chunk that has one takes its diagonal products row by row, with later rows' z left out.
 //
-// What bounds it.  128 x 2 000 x 8 heads of 64, bf16, ragged: 240 us, 3.7 TB/s of rows, where a copy reaches 4.9; rows of one
-// head lie 1 KB apart, 128 bytes each, and no reader of that order was measured above 3.9.  One sequence of 100 003 x 8 x 128, f16:
-// 15 + 180 us for the states between 64 segments, 400 for the rest: of a wave's time 61 % are waits (two barriers a chunk, and
-// chains of products behind shared memory), matrix instructions fill 30 %, shared memory is busy for 61 %.
+// What bounds it.  128 x 2 000 x 8 heads of 64, bf16, ragged: 241 us, 3.7 TB/s of rows (3.9 where all have 2 000 steps); rows of one
+// head, 128 bytes at a stride of 1 KB, can be read and written at 4.3 to 4.4, a copy reaches 4.9.  Waits are 53 % of a wave's time,
+// vector units 36 % busy, matrix units 13 %.  One sequence of 100 003 x 8 x 128, f16, 530 us: about a third for the states between 64
+// segments and their join, the rest for the rows: of a wave's time 62 % are waits (two barriers a chunk, and chains of products
+// behind shared memory), matrix instructions fill 28 %, shared memory is busy for 56 %.
 // Why 32 steps: with 64 the triangle costs twice the products and half as many segments fit; no case was faster.
 // Tried and slower: two buffers of shared memory, chunks fetched two ahead (f16 608 -> 818: registers), rows padded so that no
 // two lanes meet on a bank (conflicts halved, 534 -> 547; 16 x 2 000 x 8 x 64 bf16 training 206 -> 278).
@@ -228,7 +233,7 @@ __device__ __forceinline__ void walk_chunks(const DecayRuns& a, const DecayRun& 
     using Sh = Shape<D>;
     constexpr int NP = Type<T>::planes, C = DECAY_CHUNK, CT = C / 16, ET = Sh::et, KB = Sh::kb;
     constexpr int ROW = Sh::row, PLANE = C * ROW, N = Sh::threads, W = Sh::waves, PIECES = C * (D / 8) / N;
-    constexpr int KEEP = NP == 3 ? 2 : 1;                     // products of planes p + q <= KEEP go into the result
+    constexpr int KEEP = NP == 3 ? 2 : 1;                     // products of planes p + q <= KEEP go into the result (Precision, above)
     constexpr int PROW = C + 8, PPLANE = C * PROW;            // of the weights
     constexpr int SLOPE_PLANES = 3;
     constexpr bool OUT = !STATES_ONLY, DOT = SLOPE && OUT;

@@ -13,8 +13,9 @@
 // sixteen, by its length and the number of rows, and every lane reads 16 bytes at a time, four times before it computes.
 //   4 096 x 32 768 bf16, k = 32:      loss 59 to 86 us (4.5 to 3.1 TB/s), gradient 89 (6.0)
 //   1 023 x 131 071 f32, k = 100:     loss 117 to 153 (4.6 to 3.5), gradient 211 (5.1), where a copy of 2 GiB reaches 4.9
-//   2 047 x 50 001 bf16, k = 64:      the largest logits 62 (3.3): exponentials and comparisons fill half of the time
-//   10 000 x 5 f32 and 256 x 5 f32:   3.5, and 9.5 + 1.6 + 4.4: launches and the latency of a few dependent reductions
+//   2 047 x 50 001 bf16, k = 64:      the largest logits 63 (3.3): exponentials and comparisons fill half of the time, loads are
+//                                     waited for in the other
+//   10 000 x 5 f32 and 256 x 5 f32:   3.6, and 9.6 + 2.3 + 4.4: launches and the latency of a few dependent reductions
 #include "pxg_ops.h"
 #include <type_traits>
 
@@ -704,7 +705,7 @@ __global__ __launch_bounds__(G == 64 ? 256 : G) void k_distill_forward(const pxg
     }
 }
 
-// One workgroup, in a fixed order, eight loads ahead of the additions (4 096 rows 3.8 us, one after the other 5.6; 16 384 rows 6.2).
+// One workgroup, in a fixed order, eight loads ahead of the additions (4 096 rows 3.9 us, one after the other 5.6; 16 384 rows 6.2).
 __global__ __launch_bounds__(1024) void k_distill_sum(const float* row_loss, int64_t rows, int mean, float* loss)
 {
     constexpr int AT_ONCE = 8;

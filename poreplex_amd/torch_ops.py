@@ -124,8 +124,10 @@ def decay_attention(q, k, v, log_decay, lengths=None, initial_state=None, return
     initial_state [batch, heads, dk, dv] float32: S before the first step, 0 if None.
 
     Returns o [batch, steps, heads, dv] in v's type, or (o, S behind each sequence's last step, float32).  Differentiable in q,
-    k, v, log_decay and initial_state.  Sums and states are held in float32 whatever the tensors' type; float32 numbers of 3.38e38
-    and more count as infinite."""
+    k, v, log_decay and initial_state.  Sums and states are held in float32 whatever the tensors' type.  Products take their
+    operands in bfloat16 parts: of float32 numbers all 24 bits, less what is below 2^-24 of each term; where results are rounded to
+    half precision, 16 bits of the weights exp(log_decay * (i - j)) q_i k_j inside 32 steps and of the state before them (2^-18 of
+    each term).  float32 numbers of 3.38e38 and more count as infinite."""
     _check_decay(q, k, v, log_decay, lengths, initial_state)
     out, state = _ext().decay_attention(q, k, v, log_decay, lengths, initial_state, return_state)
     return (out, state) if return_state else out
