@@ -25,6 +25,7 @@ import os
 import socket
 import sys
 import time
+import warnings
 
 import numpy as np
 
@@ -36,6 +37,9 @@ from poreplex_amd.config import default_config  # noqa: E402
 from poreplex_amd.distributed import (gather_labels, gather_labels_start,  # noqa: E402
                                       shard_range)
 from poreplex_amd.synth import synth_batch  # noqa: E402
+
+# every process of the legs below would say so (worker processes import this file, too); the line does instead
+warnings.filterwarnings('ignore', 'this machine page-locks no memory', RuntimeWarning)
 
 # algorithmic work per read (SURVEY.md 8d / DESIGN.md "Roofline accounting")
 FLOP_SCALER = 2.0 * 2000 * (48 * 192 + 96 * 192) + 2000 * 192 * 2 + 2 * 48 * 2   # ~111.4 MFLOP
@@ -1537,6 +1541,7 @@ def main():
     if configs4 is not None:
         extra['configs4_strong'] = configs4
     extra['numa'] = numa
+    extra['arrays_stayed_pageable'] = N._warned_of_pageable         # (this process's)
 
     # ---- CPU baseline + concordance: the oracle, rank 0, bounded sample -------
     cpu = None
